@@ -10,7 +10,8 @@ library.  This Python package is host plumbing over that C ABI:
 * ``build``    -- the nvcc build recipe.
 """
 from ._lib import (  # noqa: F401
-    ACC_FP32, ACC_FP64, DENSE, PADDED, TARGET_FP32, TARGET_FP64,
+    ACC_FP32, ACC_FP64, DENSE, FP8_E4M3, FP8_E5M2, PADDED, SCALE_BLOCK, TARGET_FP32,
+    TARGET_FP64, TYPE_BF16, TYPE_FP16, TYPE_FP32,
     AutError, Workspace, check, format_id, format_info, generate, load,
     storage_bytes,
 )

@@ -29,11 +29,15 @@ STRATEGY_AUTO, STRATEGY_LDG, STRATEGY_TMA, STRATEGY_SCALAR, STRATEGY_COOPERATIVE
 (DECODER_AUTO, DECODER_DIRECT, DECODER_FULL_LUT, DECODER_FRACTION_LUT,
  DECODER_FRACTION_LUT_FUSED, DECODER_FUSED_SUM_LUT, DECODER_EX2_APPROX,
  DECODER_PREFIX_LUT, DECODER_SUBNORMAL_LUT) = range(9)
+FP8_E4M3, FP8_E5M2 = 0, 1
+TYPE_FP32, TYPE_BF16, TYPE_FP16 = 0, 1, 2
+SCALE_BLOCK = 128
 STATUS_WAIT_TIMEOUT = 1
 GEN_SIGNED_UNIT_F64, GEN_SIGNED_UNIT_F32, GEN_NORMAL, GEN_LNS_CANCEL, GEN_POSITIVE_UNIT_F64 = range(5)
 
 # C signatures: name -> (restype, argtypes)
 _i32, _u32, _u64, _dbl = C.c_int32, C.c_uint32, C.c_uint64, C.c_double
+_flt = C.c_float
 _vp, _cp = C.c_void_p, C.c_char_p
 _i32p = C.POINTER(C.c_int32)
 SIGNATURES = {
@@ -69,6 +73,12 @@ SIGNATURES = {
     "aut_encode": (_i32, [_vp, _i32, _i32, _vp, _u64, _vp, _vp]),
     "aut_generate": (_i32, [_i32, _u64, _i32, _u64, _u64, _vp, _vp]),
     "aut_generate_dot_v1": (_i32, [_i32, _u64, _i32, _i32, _u64, _u64, _u64, _vp, _vp]),
+    "aut_encode_scaled": (_i32, [_vp, _i32, _i32, _i32, _vp, _u64, _u64, _u64, _vp, _u64, _vp,
+                                 _u64, _vp]),
+    "aut_rms_norm_scaled": (_i32, [_vp, _i32, _i32, _vp, _u64, _vp, _vp, _u64, _vp, _flt, _u64,
+                                   _u64, _vp, _u64, _vp, _u64, _vp]),
+    "aut_gemm_scaled": (_i32, [_vp, _i32, _i32, _i32, _vp, _u64, _vp, _u64, _vp, _u64, _vp,
+                               _u64, _u64, _u64, _u64, _vp, _u64, _vp]),
     "aut_encode_host": (_i32, [_i32, _vp, _u64, _vp]),
     "aut_decode_host": (_i32, [_i32, _vp, _u64, _vp]),
     "aut_pack_host": (_i32, [_i32, _i32, _vp, _u64, _vp]),
@@ -181,6 +191,34 @@ class Workspace:
 
     def encode(self, fmt, layout, values_ptr, n, codes_ptr, stream=0) -> None:
         check(load().aut_encode(self.handle, fmt, layout, values_ptr, n, codes_ptr, stream))
+
+    def encode_scaled(self, code, type, block_rows, values_ptr, value_stride, rows, columns,
+                      codes_ptr, code_stride, scales_ptr, scale_stride, stream=0) -> None:
+        """Values to 8-bit codes with a scale per block of block_rows x 128
+        (strides in elements; the scale of row group R, column block b stands
+        at scales[b * scale_stride + R])."""
+        check(load().aut_encode_scaled(self.handle, code, type, block_rows, values_ptr,
+                                       value_stride, rows, columns, codes_ptr, code_stride,
+                                       scales_ptr, scale_stride, stream))
+
+    def rms_norm_scaled(self, code, type, x_ptr, x_stride, residual_ptr, residual_out_ptr,
+                        residual_stride, weight_ptr, eps, rows, columns, codes_ptr, code_stride,
+                        scales_ptr, scale_stride, stream=0) -> None:
+        """Root-mean-square norm of x + residual, encoded with a scale per row
+        and 128 columns; residual, residual_out and weight may be 0 (absent)."""
+        check(load().aut_rms_norm_scaled(self.handle, code, type, x_ptr, x_stride, residual_ptr,
+                                         residual_out_ptr, residual_stride, weight_ptr, eps,
+                                         rows, columns, codes_ptr, code_stride, scales_ptr,
+                                         scale_stride, stream))
+
+    def gemm_scaled(self, a_code, b_code, type, a_ptr, a_stride, a_scales_ptr, a_scale_stride,
+                    b_ptr, b_stride, b_scales_ptr, b_scale_stride, m, n, k, out_ptr, out_stride,
+                    stream=0) -> None:
+        """out[m, n] = a[m, k] times b[n, k] transposed, both block-scaled
+        codes: a with a scale per row, b with one per 128 rows."""
+        check(load().aut_gemm_scaled(self.handle, a_code, b_code, type, a_ptr, a_stride,
+                                     a_scales_ptr, a_scale_stride, b_ptr, b_stride, b_scales_ptr,
+                                     b_scale_stride, m, n, k, out_ptr, out_stride, stream))
 
 
 def generate_dot_v1(family: int, seed: int, parameter: int, vector_id: int, count: int,

@@ -25,6 +25,25 @@ aut_status dot_launch(aut_workspace *ws, int32_t format, int32_t layout,
                       unsigned int *status, int max_blocks_total);
 int32_t dot_supported(int32_t format, int32_t layout, int32_t accum);
 
+// The block-scaled 8-bit operators (scaled.cu, gemm_scaled.cu); sizes are not
+// zero (except k) and arguments are checked.
+aut_status encode_scaled_launch(aut_workspace *ws, int32_t code, int32_t type, int32_t block_rows,
+                                const void *values, uint64_t rows, uint64_t columns,
+                                uint64_t value_stride, void *codes, uint64_t code_stride,
+                                float *scales, uint64_t scale_stride, cudaStream_t stream);
+aut_status rms_norm_scaled_launch(aut_workspace *ws, int32_t code, int32_t type, const void *x,
+                                  uint64_t x_stride, const void *residual, void *residual_out,
+                                  uint64_t residual_stride, const void *weight, float eps,
+                                  uint64_t rows, uint64_t columns, void *codes,
+                                  uint64_t code_stride, float *scales, uint64_t scale_stride,
+                                  cudaStream_t stream);
+aut_status gemm_scaled_launch(aut_workspace *ws, int32_t a_code, int32_t b_code, int32_t type,
+                              const void *a, uint64_t a_stride, const float *a_scales,
+                              uint64_t a_scale_stride, const void *b, uint64_t b_stride,
+                              const float *b_scales, uint64_t b_scale_stride, uint64_t m,
+                              uint64_t n, uint64_t k, void *out, uint64_t out_stride,
+                              cudaStream_t stream);
+
 // ---- format registry ----------------------------------------------------------
 // Ids 0..10 are the formats with fused DOT kernels (autdot.h); the rest follow
 // the reference's registries (storage_formats.hpp:110-262,
@@ -794,6 +813,134 @@ aut_status aut_generate_dot_v1(int32_t family, uint64_t seed, int32_t parameter,
   if (n > 0 && out == nullptr) return fail(AUT_ERR_INVALID_ARGUMENT, "out is NULL");
   return launch_generate_dot_v1(family, seed, parameter, vector_id, count, first, n, out,
                                 static_cast<cudaStream_t>(stream));
+}
+
+// Checks of the block-scaled operators' arguments: each returns AUT_OK or the
+// failure of the first argument that does not hold.
+static aut_status check_code(int32_t code) {
+  if (code != AUT_FP8_E4M3 && code != AUT_FP8_E5M2)
+    return fail(AUT_ERR_INVALID_ARGUMENT, "code must be E4M3 or E5M2");
+  return AUT_OK;
+}
+
+static aut_status check_type(int32_t type) {
+  if (type != AUT_TYPE_FP32 && type != AUT_TYPE_BF16 && type != AUT_TYPE_FP16)
+    return fail(AUT_ERR_INVALID_ARGUMENT, "type must be FP32, BF16 or FP16");
+  return AUT_OK;
+}
+
+static uint64_t size_of_type(int32_t type) { return type == AUT_TYPE_FP32 ? 4 : 2; }
+
+static aut_status check_matrix(const char *name, const void *pointer, uint64_t rows,
+                               uint64_t columns, uint64_t stride, uint64_t size) {
+  const std::string what(name);
+  if (pointer == nullptr) return fail(AUT_ERR_INVALID_ARGUMENT, what + " is NULL");
+  if (reinterpret_cast<uintptr_t>(pointer) % size != 0)
+    return fail(AUT_ERR_INVALID_ARGUMENT, what + " is not aligned to its elements");
+  if (rows > 1 && stride < columns)
+    return fail(AUT_ERR_INVALID_ARGUMENT, what + ": stride smaller than one row");
+  if (rows > 1 && stride > (uint64_t{1} << 53) / size / (rows - 1))
+    return fail(AUT_ERR_TOO_LARGE, what + ": matrix larger than 2^53 bytes");
+  return AUT_OK;
+}
+
+// The scales of `rows` x `columns` codes in groups of block_rows.
+static aut_status check_scales(const char *name, const float *scales, uint64_t rows,
+                               uint64_t columns, uint64_t block_rows, uint64_t stride) {
+  return check_matrix(name, scales, (columns + AUT_SCALE_BLOCK - 1) / AUT_SCALE_BLOCK,
+                      (rows + block_rows - 1) / block_rows, stride, sizeof(float));
+}
+
+static aut_status check_sizes(uint64_t a, uint64_t b, uint64_t c) {
+  if (a > 0x7fffffffull || b > 0x7fffffffull || c > 0x7fffffffull)
+    return fail(AUT_ERR_TOO_LARGE, "at most 2^31 - 1 rows and columns");
+  return AUT_OK;
+}
+
+#define AUT_CHECK(expr)                    \
+  do {                                     \
+    const aut_status aut_st_ = (expr);     \
+    if (aut_st_ != AUT_OK) return aut_st_; \
+  } while (0)
+
+aut_status aut_encode_scaled(aut_workspace *ws, int32_t code, int32_t type, int32_t block_rows,
+                             const void *values, uint64_t value_stride, uint64_t rows,
+                             uint64_t columns, void *codes, uint64_t code_stride, float *scales,
+                             uint64_t scale_stride, void *stream) {
+  clear_error();
+  if (ws == nullptr) return fail(AUT_ERR_INVALID_ARGUMENT, "workspace is NULL");
+  AUT_CHECK(check_code(code));
+  AUT_CHECK(check_type(type));
+  if (block_rows != 1 && block_rows != AUT_SCALE_BLOCK)
+    return fail(AUT_ERR_INVALID_ARGUMENT, "block_rows must be 1 or 128");
+  if (rows == 0 || columns == 0) return AUT_OK;
+  AUT_CHECK(check_sizes(rows, columns, 0));
+  AUT_CHECK(check_matrix("values", values, rows, columns, value_stride, size_of_type(type)));
+  AUT_CHECK(check_matrix("codes", codes, rows, columns, code_stride, 1));
+  AUT_CHECK(check_scales("scales", scales, rows, columns, block_rows, scale_stride));
+  device_scope scope(ws->device);
+  AUT_CUDA_TRY(scope.err);
+  return encode_scaled_launch(ws, code, type, block_rows, values, rows, columns, value_stride,
+                              codes, code_stride, scales, scale_stride,
+                              static_cast<cudaStream_t>(stream));
+}
+
+aut_status aut_rms_norm_scaled(aut_workspace *ws, int32_t code, int32_t type, const void *x,
+                               uint64_t x_stride, const void *residual, void *residual_out,
+                               uint64_t residual_stride, const void *weight, float eps,
+                               uint64_t rows, uint64_t columns, void *codes,
+                               uint64_t code_stride, float *scales, uint64_t scale_stride,
+                               void *stream) {
+  clear_error();
+  if (ws == nullptr) return fail(AUT_ERR_INVALID_ARGUMENT, "workspace is NULL");
+  AUT_CHECK(check_code(code));
+  AUT_CHECK(check_type(type));
+  if (!(eps >= 0.0f)) return fail(AUT_ERR_INVALID_ARGUMENT, "eps must not be negative");
+  if (rows == 0 || columns == 0) return AUT_OK;
+  AUT_CHECK(check_sizes(rows, columns, 0));
+  const uint64_t size = size_of_type(type);
+  AUT_CHECK(check_matrix("x", x, rows, columns, x_stride, size));
+  if (residual != nullptr)
+    AUT_CHECK(check_matrix("residual", residual, rows, columns, residual_stride, size));
+  if (residual_out != nullptr)
+    AUT_CHECK(check_matrix("residual_out", residual_out, rows, columns, residual_stride, size));
+  if (residual_out == x && rows > 1 && x_stride != residual_stride)
+    return fail(AUT_ERR_INVALID_ARGUMENT, "residual_out is x with another stride");
+  if (weight != nullptr) AUT_CHECK(check_matrix("weight", weight, 1, columns, columns, size));
+  AUT_CHECK(check_matrix("codes", codes, rows, columns, code_stride, 1));
+  AUT_CHECK(check_scales("scales", scales, rows, columns, 1, scale_stride));
+  device_scope scope(ws->device);
+  AUT_CUDA_TRY(scope.err);
+  return rms_norm_scaled_launch(ws, code, type, x, x_stride, residual, residual_out,
+                                residual_stride, weight, eps, rows, columns, codes, code_stride,
+                                scales, scale_stride, static_cast<cudaStream_t>(stream));
+}
+
+aut_status aut_gemm_scaled(aut_workspace *ws, int32_t a_code, int32_t b_code, int32_t type,
+                           const void *a, uint64_t a_stride, const float *a_scales,
+                           uint64_t a_scale_stride, const void *b, uint64_t b_stride,
+                           const float *b_scales, uint64_t b_scale_stride, uint64_t m,
+                           uint64_t n, uint64_t k, void *out, uint64_t out_stride,
+                           void *stream) {
+  clear_error();
+  if (ws == nullptr) return fail(AUT_ERR_INVALID_ARGUMENT, "workspace is NULL");
+  AUT_CHECK(check_code(a_code));
+  AUT_CHECK(check_code(b_code));
+  AUT_CHECK(check_type(type));
+  if (m == 0 || n == 0) return AUT_OK;
+  AUT_CHECK(check_sizes(m, n, k));
+  if (k != 0) {
+    AUT_CHECK(check_matrix("a", a, m, k, a_stride, 1));
+    AUT_CHECK(check_scales("a_scales", a_scales, m, k, 1, a_scale_stride));
+    AUT_CHECK(check_matrix("b", b, n, k, b_stride, 1));
+    AUT_CHECK(check_scales("b_scales", b_scales, n, k, AUT_SCALE_BLOCK, b_scale_stride));
+  }
+  AUT_CHECK(check_matrix("out", out, m, n, out_stride, size_of_type(type)));
+  device_scope scope(ws->device);
+  AUT_CUDA_TRY(scope.err);
+  return gemm_scaled_launch(ws, a_code, b_code, type, a, a_stride, a_scales, a_scale_stride, b,
+                            b_stride, b_scales, b_scale_stride, m, n, k, out, out_stride,
+                            static_cast<cudaStream_t>(stream));
 }
 
 aut_status aut_encode_host(int32_t format, const double *values, uint64_t n,

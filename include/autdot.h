@@ -114,6 +114,17 @@ enum {
                                    e8m5) */
 };
 
+/* Codes of the block-scaled 8-bit operators: the OCP 8-bit floats E4M3
+ * (largest value 448, one NaN magnitude, no infinities) and E5M2 (largest
+ * finite value 57344). */
+enum { AUT_FP8_E4M3 = 0, AUT_FP8_E5M2 = 1 };
+
+/* Element types of the values the block-scaled operators read and write. */
+enum { AUT_TYPE_FP32 = 0, AUT_TYPE_BF16 = 1, AUT_TYPE_FP16 = 2 };
+
+/* Columns (and, for weights, rows) that share one scale. */
+#define AUT_SCALE_BLOCK 128
+
 /* Sticky device status bits reported by aut_workspace_status(). */
 enum {
   AUT_STATUS_WAIT_TIMEOUT = 1 /* a bounded pipeline wait gave up; the
@@ -320,6 +331,68 @@ aut_status aut_generate(int32_t kind, uint64_t seed, int32_t vector_id,
 aut_status aut_generate_dot_v1(int32_t family, uint64_t seed, int32_t parameter,
                                int32_t vector_id, uint64_t count, uint64_t first,
                                uint64_t n, float *out, void *stream);
+
+/* ---- block-scaled 8-bit codes --------------------------------------------- */
+/* A scaled matrix is a row-major matrix of 8-bit codes (AUT_FP8_*), row r at
+ * codes + r * code_stride, with one FP32 scale per block of 128 columns of
+ * one row (activations) or of 128 rows (weights): the scale of row group R
+ * and column block b is scales[b * scale_stride + R].  The last block of a
+ * row and the last row group may be shorter.  A value is its code's value
+ * times its block's scale.  No counterpart in the reference, whose narrow
+ * formats carry no scale.
+ *
+ * All strides are in elements.  Values and scales are aligned to their own
+ * size; any stride and any alignment of the codes is served.  A stride is at
+ * least the length of what it steps over (it is not looked at where there is
+ * only one row, or one column block).  At most 2^31 - 1 rows and columns, and
+ * 2^53 bytes per matrix.  Outputs may not overlap inputs, except as said. */
+
+/* Encodes values[rows][columns] (AUT_TYPE_*) with one scale per block of
+ * block_rows (1 or 128) x 128:
+ *   scale = max(largest finite |x| of the block / F, 2^-126), F the format's
+ *           largest finite value; code = x / scale (FP32) rounded to nearest
+ *           even; infinities and NaN become the NaN code.
+ * codes may not overlap values.  rows = 0 or columns = 0 does nothing. */
+aut_status aut_encode_scaled(aut_workspace *ws, int32_t code, int32_t type,
+                             int32_t block_rows, const void *values,
+                             uint64_t value_stride, uint64_t rows,
+                             uint64_t columns, void *codes,
+                             uint64_t code_stride, float *scales,
+                             uint64_t scale_stride, void *stream);
+
+/* Root-mean-square norm with the residual's addition, encoded by rows:
+ *   h = x + residual (h = x for residual = NULL), in FP32;
+ *   residual_out = h rounded to `type` (not written for NULL);
+ *   y = h / sqrt(mean(h^2) + eps) * weight (no factor for weight = NULL);
+ *   y encoded as by aut_encode_scaled with block_rows = 1.
+ * x, residual, residual_out and weight[columns] have the type `type`;
+ * residual and residual_out share residual_stride.  residual_out may be
+ * residual itself, or x where both strides are equal; it may not overlap
+ * them otherwise.  The mean is summed in FP32. */
+aut_status aut_rms_norm_scaled(aut_workspace *ws, int32_t code, int32_t type,
+                               const void *x, uint64_t x_stride,
+                               const void *residual, void *residual_out,
+                               uint64_t residual_stride, const void *weight,
+                               float eps, uint64_t rows, uint64_t columns,
+                               void *codes, uint64_t code_stride,
+                               float *scales, uint64_t scale_stride,
+                               void *stream);
+
+/* out[i * out_stride + j] = sum_c value of a[i][c] * value of b[j][c] for
+ * i < m, j < n, c < k, rounded once to `type` (AUT_TYPE_*).  a holds codes
+ * a_code with one scale per row (block_rows = 1), b (the weights, one row per
+ * output column) codes b_code with block_rows = 128.  The codes' products are
+ * summed in FP32 within a block of 128 and then, times both scales, over the
+ * blocks.  Codes beyond column k are never read into the product.  Operands
+ * whose pointers and strides are multiples of 16 bytes take the vectorised
+ * paths.  m = 0 or n = 0 does nothing; k = 0 writes zeros. */
+aut_status aut_gemm_scaled(aut_workspace *ws, int32_t a_code, int32_t b_code,
+                           int32_t type, const void *a, uint64_t a_stride,
+                           const float *a_scales, uint64_t a_scale_stride,
+                           const void *b, uint64_t b_stride,
+                           const float *b_scales, uint64_t b_scale_stride,
+                           uint64_t m, uint64_t n, uint64_t k, void *out,
+                           uint64_t out_stride, void *stream);
 
 /* ---- host codecs (the host half of storage::encode/decode) -------------- */
 aut_status aut_encode_host(int32_t format, const double *values, uint64_t n,

@@ -1,0 +1,46 @@
+"""The 64-bit checker of the block-scaled operators against torch's 8-bit
+floats, and the refusals of the C entry points that need no GPU."""
+import numpy as np
+import pytest
+import torch
+
+import scaled_ref as ref
+
+TORCH = {ref.E4M3: torch.float8_e4m3fn, ref.E5M2: torch.float8_e5m2}
+
+
+@pytest.mark.parametrize("code", [ref.E4M3, ref.E5M2])
+def test_code_values(code):
+    want = torch.arange(256, dtype=torch.int16).to(torch.uint8).view(TORCH[code]).double().numpy()
+    np.testing.assert_array_equal(ref.code_values(code), want)
+
+
+@pytest.mark.parametrize("code", [ref.E4M3, ref.E5M2])
+def test_rounding(code):
+    v = ref.code_values(code)
+    v = np.unique(v[np.isfinite(v)])
+    ties = (v[1:] + v[:-1]) / 2
+    x = np.concatenate([v, ties, np.nextafter(ties.astype(np.float32), np.float32(np.inf)),
+                        np.random.default_rng(3).standard_normal(4096) * 20])
+    x = x.astype(np.float32)
+    want = torch.from_numpy(x).clamp(-ref.LARGEST[code], ref.LARGEST[code]).to(TORCH[code])
+    np.testing.assert_array_equal(ref.round_to_code(x, code), want.double().numpy())
+
+
+def test_scale_layout():
+    x = np.ones((130, 300), np.float32)
+    x[129, 299] = 448 * 4
+    s = ref.scales_of(x, ref.E4M3, 128)
+    assert s.shape == (3, 2) and s[2, 1] == 4 and s[2, 0] == np.float32(1) / np.float32(448)
+    assert ref.spread(s, 130, 300, 128)[129, 299] == 4
+
+
+def test_entry_points_refuse_a_missing_workspace(autlib):
+    from accessor_universal_test_b200 import _lib
+    bad = _lib.AUT_ERR_INVALID_ARGUMENT
+    assert autlib.aut_encode_scaled(None, 0, 0, 1, None, 0, 0, 0, None, 0, None, 0, None) == bad
+    assert autlib.aut_rms_norm_scaled(None, 0, 0, None, 0, None, None, 0, None, 0.0, 0, 0, None,
+                                      0, None, 0, None) == bad
+    assert autlib.aut_gemm_scaled(None, 0, 0, 0, None, 0, None, 0, None, 0, None, 0, 0, 0, 0,
+                                  None, 0, None) == bad
+    assert b"workspace" in autlib.aut_last_error()
