@@ -1,29 +1,9 @@
 // gemm_scaled.cu -- aut_gemm_scaled: the product of two matrices of
 // block-scaled 8-bit codes.
-#include "internal.hpp"
-#include "dot_device.cuh"
-#include "scaled_device.cuh"
+#include "gemm_scaled.cuh"
 
 namespace aut::scaled {
 namespace {
-
-struct gemm_params {
-  const uint8_t *a; // m rows of k codes, one scale per row and 128 columns
-  const uint8_t *b; // n rows of k codes, one scale per 128 rows and 128 columns
-  const float *a_scales, *b_scales;
-  void *out;
-  uint64_t a_stride, b_stride, a_scale_stride, b_scale_stride, out_stride;
-  uint64_t m, n, k;
-  int type;
-};
-
-__device__ __forceinline__ void store_out(const gemm_params &p, uint64_t i, uint64_t j, float v) {
-  const uint64_t at = i * p.out_stride + j;
-  if (p.type == AUT_TYPE_FP32) static_cast<float *>(p.out)[at] = v;
-  else if (p.type == AUT_TYPE_BF16)
-    static_cast<__nv_bfloat16 *>(p.out)[at] = narrow<__nv_bfloat16>(v);
-  else static_cast<__half *>(p.out)[at] = narrow<__half>(v);
-}
 
 // Sixteen codes of a row from column c on; codes at or beyond column k read
 // as zero (what a caller's row padding holds never enters the product).
@@ -138,8 +118,8 @@ aut_status launch(void (*kernel)(Params), uint64_t grid, int max_grid, int threa
 
 template <int ACode, int BCode>
 aut_status gemm_typed(aut_workspace *ws, const gemm_params &p, cudaStream_t stream) {
-  const bool aligned = reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && p.a_stride % 16 == 0 &&
-                       reinterpret_cast<uintptr_t>(p.b) % 16 == 0 && p.b_stride % 16 == 0;
+  const bool aligned = aligned_operands(p);
+  if (aligned && p.m > 16 && p.k > 0) return gemm_tiles(ws, p, ACode, BCode, stream);
   const uint64_t tasks = (p.n + 15) / 16 * ((p.m + 7) / 8);
   return launch(aligned ? rows_kernel<ACode, BCode, true> : rows_kernel<ACode, BCode, false>,
                 tasks, 64 * ws->max_blocks, 256, p, stream);
