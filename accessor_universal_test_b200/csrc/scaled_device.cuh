@@ -49,13 +49,6 @@ template <int Code> __device__ __forceinline__ uint32_t codes_of(float lo, float
   return r;
 }
 
-// The scale of a block whose largest finite magnitude is `largest`: at least
-// 2^-126, so that its reciprocal is finite and a block of zeros needs no case
-// of its own.
-template <int Code> __device__ __forceinline__ float scale_of(float largest) {
-  return fmaxf(__fdiv_rn(largest, largest_code<Code>()), 1.17549435e-38f);
-}
-
 // x / scale rounded to FP32, from the block's one reciprocal: Markstein's
 // correction step (the residual x - q * scale is exact in one FMA) makes the
 // product with the rounded reciprocal the correctly rounded quotient, so a
@@ -66,6 +59,14 @@ template <int Code> __device__ __forceinline__ float scale_of(float largest) {
 __device__ __forceinline__ float quotient(float x, float scale, float reciprocal) {
   const float q = x * reciprocal;
   return fmaf(fmaf(-q, scale, x), reciprocal, q);
+}
+
+// The scale of a block whose largest finite magnitude is `largest`: at least
+// 2^-126, so that its reciprocal is finite and a block of zeros needs no case
+// of its own.
+template <int Code> __device__ __forceinline__ float scale_of(float largest) {
+  constexpr float f = largest_code<Code>(), reciprocal = 1.0f / f;
+  return fmaxf(quotient(largest, f, reciprocal), 1.17549435e-38f);
 }
 
 // |v| for a block's largest magnitude: infinities and NaN do not count.
