@@ -4,7 +4,7 @@
 #include "dot_device.cuh"
 #include "scaled_device.cuh"
 
-#include <cstring>
+#include <algorithm>
 
 namespace aut::scaled {
 namespace {
@@ -31,7 +31,7 @@ struct norm_params {
 // ---- a warp's chunk: 256 columns, eight values a lane ---------------------------
 // Vec: lane l holds the columns 8 l .. 8 l + 7, one or two 16-byte loads and one
 // 8-byte store of codes; 16 lanes share a scale.  Needs rows of values on
-// 16-byte and rows of codes on 8-byte boundaries.
+// 16-byte and rows of codes on 8-byte boundaries, and a multiple of 8 columns.
 // Not Vec: lane l holds the columns l + 32 j, so that any alignment is read and
 // written in whole lines; all 32 lanes share the scale of four values.
 template <bool Vec>
@@ -39,137 +39,158 @@ __device__ __forceinline__ uint32_t column_of(uint32_t chunk, int lane, int j) {
   return Vec ? (chunk * 32 + lane) * 8 + j : chunk * 256 + j * 32 + lane;
 }
 
-__device__ __forceinline__ void widen_pair(__nv_bfloat162 p, float &a, float &b) {
-  const float2 f = __bfloat1622float2(p);
-  a = f.x;
-  b = f.y;
+__device__ __forceinline__ float2 widen_pair(uint32_t w, __nv_bfloat16) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
-__device__ __forceinline__ void widen_pair(__half2 p, float &a, float &b) {
-  const float2 f = __half22float2(p);
-  a = f.x;
-  b = f.y;
+__device__ __forceinline__ float2 widen_pair(uint32_t w, __half) {
+  return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+__device__ __forceinline__ uint32_t narrow_pair(float2 v, __nv_bfloat16) {
+  const __nv_bfloat162 n = __float22bfloat162_rn(v);
+  return *reinterpret_cast<const uint32_t *>(&n);
+}
+__device__ __forceinline__ uint32_t narrow_pair(float2 v, __half) {
+  const __half2 n = __float22half2_rn(v);
+  return *reinterpret_cast<const uint32_t *>(&n);
 }
 
-template <class T> struct pair_of;
-template <> struct pair_of<__nv_bfloat16> { using type = __nv_bfloat162; };
-template <> struct pair_of<__half> { using type = __half2; };
+// Eight values as they stand in memory.
+template <class T> struct raw_chunk { uint32_t w[2 * sizeof(T)]; };
+template <size_t Size> struct raw_word { using type = uint32_t; };
+template <> struct raw_word<2> { using type = uint16_t; };
 
-__device__ __forceinline__ void load_eight(const float *x, float (&v)[8]) {
-  const float4 a = reinterpret_cast<const float4 *>(x)[0];
-  const float4 b = reinterpret_cast<const float4 *>(x)[1];
-  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-  v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-}
-template <class T> __device__ __forceinline__ void load_eight(const T *x, float (&v)[8]) {
-  const uint4 u = *reinterpret_cast<const uint4 *>(x);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+__device__ __forceinline__ void widen_chunk(const raw_chunk<float> &r, float2 (&v)[4]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    widen_pair(*reinterpret_cast<const typename pair_of<T>::type *>(&w[i]), v[2 * i],
-               v[2 * i + 1]);
+  for (int j = 0; j < 4; ++j)
+    v[j] = make_float2(__uint_as_float(r.w[2 * j]), __uint_as_float(r.w[2 * j + 1]));
+}
+template <class T>
+__device__ __forceinline__ void widen_chunk(const raw_chunk<T> &r, float2 (&v)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = widen_pair(r.w[j], T{});
 }
 
-__device__ __forceinline__ void store_eight(float *x, const float (&v)[8]) {
-  reinterpret_cast<float4 *>(x)[0] = make_float4(v[0], v[1], v[2], v[3]);
-  reinterpret_cast<float4 *>(x)[1] = make_float4(v[4], v[5], v[6], v[7]);
+__device__ __forceinline__ void store_eight(float *x, const float2 (&v)[4]) {
+  reinterpret_cast<float4 *>(x)[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+  reinterpret_cast<float4 *>(x)[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
 }
-template <class T> __device__ __forceinline__ void store_eight(T *x, const float (&v)[8]) {
-  T n[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) n[j] = narrow<T>(v[j]);
-  uint4 u;
-  memcpy(&u, n, 16);
-  *reinterpret_cast<uint4 *>(x) = u;
+template <class T> __device__ __forceinline__ void store_eight(T *x, const float2 (&v)[4]) {
+  *reinterpret_cast<uint4 *>(x) = make_uint4(narrow_pair(v[0], T{}), narrow_pair(v[1], T{}),
+                                             narrow_pair(v[2], T{}), narrow_pair(v[3], T{}));
 }
 
 // The chunk's values of a row; columns beyond the row read as zero.
 template <bool Vec, class T>
-__device__ __forceinline__ void load_chunk(const T *row, uint32_t chunk, int lane,
-                                           uint32_t columns, float (&v)[8]) {
-  if (Vec && column_of<Vec>(chunk, lane, 8) <= columns) {
-    load_eight(row + column_of<Vec>(chunk, lane, 0), v);
-    return;
-  }
+__device__ __forceinline__ raw_chunk<T> load_raw(const T *row, uint32_t chunk, int lane,
+                                                 uint32_t columns) {
+  raw_chunk<T> r;
+  const uint32_t c0 = column_of<Vec>(chunk, lane, 0);
+  if constexpr (Vec) {
+    const uint4 *x = reinterpret_cast<const uint4 *>(row + c0);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t c = column_of<Vec>(chunk, lane, j);
-    v[j] = c < columns ? widen(row[c]) : 0.0f;
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+      const uint4 u = c0 < columns ? x[i] : make_uint4(0u, 0u, 0u, 0u);
+      r.w[4 * i] = u.x, r.w[4 * i + 1] = u.y, r.w[4 * i + 2] = u.z, r.w[4 * i + 3] = u.w;
+    }
+  } else {
+    using word = typename raw_word<sizeof(T)>::type;
+    const word *x = reinterpret_cast<const word *>(row + c0);
+    uint32_t bits[8];
+    if (chunk * 256 + 256 <= columns) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) bits[j] = x[32 * j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) bits[j] = c0 + 32 * j < columns ? x[32 * j] : word{0};
+    }
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(2 * sizeof(T)); ++i)
+      r.w[i] = sizeof(T) == 4 ? bits[i] : bits[2 * i % 8] | bits[(2 * i + 1) % 8] << 16;
   }
+  return r;
+}
+
+template <bool Vec, class T>
+__device__ __forceinline__ void load_chunk(const T *row, uint32_t chunk, int lane,
+                                           uint32_t columns, float2 (&v)[4]) {
+  widen_chunk(load_raw<Vec>(row, chunk, lane, columns), v);
 }
 
 template <bool Vec, class T>
 __device__ __forceinline__ void store_chunk(T *row, uint32_t chunk, int lane, uint32_t columns,
-                                            const float (&v)[8]) {
-  if (Vec && column_of<Vec>(chunk, lane, 8) <= columns) {
-    store_eight(row + column_of<Vec>(chunk, lane, 0), v);
-    return;
-  }
+                                            const float2 (&v)[4]) {
+  const uint32_t c0 = column_of<Vec>(chunk, lane, 0);
+  if constexpr (Vec) {
+    if (c0 < columns) store_eight(row + c0, v);
+  } else {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t c = column_of<Vec>(chunk, lane, j);
-    if (c < columns) row[c] = narrow<T>(v[j]);
+    for (int j = 0; j < 8; ++j)
+      if (c0 + 32 * j < columns)
+        row[c0 + 32 * j] = narrow<T>(j % 2 == 0 ? v[j / 2].x : v[j / 2].y);
   }
 }
 
-template <int Code> __device__ __forceinline__ uint32_t four_codes(const float *q) {
-  return __byte_perm(codes_of<Code>(q[0], q[1]), codes_of<Code>(q[2], q[3]), 0x5410);
+template <int Code> __device__ __forceinline__ uint32_t four_codes(float2 a, float2 b) {
+  return __byte_perm(codes_of<Code>(a.x, a.y), codes_of<Code>(b.x, b.y), 0x5410);
 }
 
-// Largest magnitude of the eight values' block or blocks (Vec: m[0]; else
-// m[h] for the values 4 h ..).
-template <bool Vec, bool Finite>
-__device__ __forceinline__ void largest_of(const float (&v)[8], float (&m)[2]) {
-  m[0] = m[1] = 0.0f;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    float &to = m[Vec ? 0 : j / 4];
-    to = fmaxf(to, Finite ? finite_magnitude(v[j]) : fabsf(v[j]));
-  }
-#pragma unroll
-  for (int d = Vec ? 8 : 16; d > 0; d >>= 1) {
-    m[0] = fmaxf(m[0], __shfl_xor_sync(0xffffffffu, m[0], d));
-    if (!Vec) m[1] = fmaxf(m[1], __shfl_xor_sync(0xffffffffu, m[1], d));
-  }
+// Largest magnitude of four values (not NaN, which is passed over; infinite
+// if one of them is).
+__device__ __forceinline__ float largest_of(float2 a, float2 b) {
+  return fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y)));
+}
+
+// Takes infinities out of a value's block: they encode as NaN and do not
+// count for the scale.
+__device__ __forceinline__ float without_infinity(float v) {
+  return fabsf(v) <= 3.40282347e38f ? v : __int_as_float(0x7fffffff);
 }
 
 // Encodes the chunk: codes into the row, scales into scales[block * stride].
 // All lanes of the warp take part.
 template <int Code, bool Vec>
-__device__ __forceinline__ void encode_chunk(const float (&v)[8], uint32_t chunk, int lane,
+__device__ __forceinline__ void encode_chunk(float2 (&v)[4], uint32_t chunk, int lane,
                                              uint32_t columns, uint8_t *row, float *scales,
                                              uint64_t scale_stride) {
-  // fmaxf passes over NaN; an infinity shows in the maximum, and only then
-  // are the values looked at again without it.
-  float m[2];
-  largest_of<Vec, false>(v, m);
-  if (__any_sync(0xffffffffu, fmaxf(m[0], m[1]) > 3.40282347e38f)) largest_of<Vec, true>(v, m);
-  float q[8];
+  constexpr int kHalves = Vec ? 1 : 2;
+  float m[2] = {largest_of(v[0], v[1]), largest_of(v[2], v[3])};
+  if (Vec) m[0] = m[1] = fmaxf(m[0], m[1]);
+  // Rare, and not worth a test for every value: an infinity.
+  if (__any_sync(0xffffffffu, fmaxf(m[0], m[1]) > 3.40282347e38f)) {
 #pragma unroll
-  for (int h = 0; h < (Vec ? 1 : 2); ++h) {
-    const float scale = scale_of<Code>(m[h]);
-    const float reciprocal = __frcp_rn(scale);
-    const uint32_t block = chunk * 2 + (Vec ? lane / 16 : h);
-    if ((Vec ? lane % 16 : lane) == 0 && block * kBlock < columns)
-      scales[block * scale_stride] = scale;
-#pragma unroll
-    for (int j = h * 4; j < (Vec ? 8 : h * 4 + 4); ++j) q[j] = quotient(v[j], scale, reciprocal);
+    for (int j = 0; j < 4; ++j)
+      v[j] = make_float2(without_infinity(v[j].x), without_infinity(v[j].y));
+    m[0] = largest_of(v[0], v[1]), m[1] = largest_of(v[2], v[3]);
+    if (Vec) m[0] = fmaxf(m[0], m[1]);
   }
-  const uint32_t lo = four_codes<Code>(q), hi = four_codes<Code>(q + 4);
-  if (Vec && column_of<Vec>(chunk, lane, 8) <= columns) {
-    *reinterpret_cast<uint2 *>(row + column_of<Vec>(chunk, lane, 0)) = make_uint2(lo, hi);
-    return;
-  }
+  uint32_t codes[2];
+  block_scale s;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t c = column_of<Vec>(chunk, lane, j);
-    if (c < columns) row[c] = static_cast<uint8_t>((j < 4 ? lo : hi) >> (8 * (j % 4)));
+  for (int h = 0; h < 2; ++h) {
+    if (h < kHalves) {
+      s = scale_of<Code>(Vec ? half_warp_max(m[h], lane) : warp_max(m[h]));
+      const uint32_t block = chunk * 2 + (Vec ? lane / 16 : h);
+      if ((Vec ? lane % 16 : lane) == 0 && block * kBlock < columns)
+        scales[block * scale_stride] = s.scale;
+    }
+    codes[h] = four_codes<Code>(quotient(v[2 * h], s), quotient(v[2 * h + 1], s));
+  }
+  const uint32_t c0 = column_of<Vec>(chunk, lane, 0);
+  if constexpr (Vec) {
+    if (c0 < columns) *reinterpret_cast<uint2 *>(row + c0) = make_uint2(codes[0], codes[1]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c0 + 32 * j < columns)
+        row[c0 + 32 * j] = static_cast<uint8_t>(codes[j / 4] >> (8 * (j % 4)));
   }
 }
 
 // ---- encode by rows ---------------------------------------------------------------
-// A block takes 256 columns of 16 rows, a warp two of the rows, both loaded
-// before either is encoded.  The rows of a block are neighbours, so the scales
-// of one column block fill whole lines.
+// Block (c, y) takes chunk c of the row groups y, y + gridDim.y, ... of 16
+// rows, a warp two rows of a group; the next group's values are loaded before
+// this one's are encoded, so loads are under way all the time.  The rows of a
+// group are neighbours: the scales of one column block fill whole lines.
 constexpr int kEncodeRows = 16;
 
 template <int Type, int Code, bool Vec>
@@ -179,92 +200,175 @@ __global__ void __launch_bounds__(256) encode_rows_kernel(const encode_params p)
   aut::dev::pdl_release();
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
   const uint32_t columns = static_cast<uint32_t>(p.columns);
-  const uint32_t chunks = (columns + 255) / 256;
-  const uint32_t chunk = blockIdx.x % chunks;
-  const uint64_t first = uint64_t{blockIdx.x / chunks} * kEncodeRows + warp;
-  float v[2][8];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (first + 8 * i < p.rows)
-      load_chunk<Vec>(static_cast<const T *>(p.x) + (first + 8 * i) * p.x_stride, chunk, lane,
-                      columns, v[i]);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint64_t row = first + 8 * i;
-    if (row < p.rows)
-      encode_chunk<Code, Vec>(v[i], chunk, lane, columns, p.codes + row * p.code_stride,
-                              p.scales + row, p.scale_stride);
+  const uint32_t chunk = blockIdx.x;
+  const uint64_t step = uint64_t{gridDim.y} * kEncodeRows;
+  const uint64_t first = uint64_t{blockIdx.y} * kEncodeRows + warp;
+  const T *x = static_cast<const T *>(p.x) + first * p.x_stride;
+  uint8_t *codes = p.codes + first * p.code_stride;
+  const uint64_t x_step = step * p.x_stride, code_step = step * p.code_stride;
+  raw_chunk<T> next[2];
+  if (first < p.rows) next[0] = load_raw<Vec>(x, chunk, lane, columns);
+  if (first + 8 < p.rows) next[1] = load_raw<Vec>(x + 8 * p.x_stride, chunk, lane, columns);
+  for (uint64_t row = first; row < p.rows; row += step, codes += code_step) {
+    const bool two = row + 8 < p.rows;
+    float2 v[2][4];
+    widen_chunk(next[0], v[0]);
+    widen_chunk(next[1], v[1]);
+    x += x_step;
+    if (row + step < p.rows) next[0] = load_raw<Vec>(x, chunk, lane, columns);
+    if (row + step + 8 < p.rows) next[1] = load_raw<Vec>(x + 8 * p.x_stride, chunk, lane, columns);
+    encode_chunk<Code, Vec>(v[0], chunk, lane, columns, codes, p.scales + row, p.scale_stride);
+    if (two)
+      encode_chunk<Code, Vec>(v[1], chunk, lane, columns, codes + 8 * p.code_stride,
+                              p.scales + row + 8, p.scale_stride);
   }
 }
 
 // ---- encode by tiles of 128 x 128 ----------------------------------------------------
-// A block holds its tile in registers, 32 values a thread, so the tile is read
-// once.  Vec: lane l holds the columns 4 l ..; else l + 32 j (see above).
-template <class T> __device__ __forceinline__ void load_four(const T *x, float *v) {
-  const uint2 u = *reinterpret_cast<const uint2 *>(x);
-  widen_pair(*reinterpret_cast<const typename pair_of<T>::type *>(&u.x), v[0], v[1]);
-  widen_pair(*reinterpret_cast<const typename pair_of<T>::type *>(&u.y), v[2], v[3]);
+// A block holds a tile in registers (16 a thread: 32 values of 16 bits, 16 of
+// 32), so the tile is read once, and loads its next one before it encodes this
+// one.  Vec: lane l holds the columns 4 l .., a multiple of 4 in all; else
+// l + 32 j (see above).
+template <class T> struct tile_of {
+  static constexpr int kThreads = sizeof(T) == 4 ? 1024 : 512;
+  static constexpr int kWarps = kThreads / 32;
+  static constexpr int kRows = kBlock / kWarps; // of each warp
+};
+// Four values of a row.
+template <class T> struct raw_four { uint32_t w[sizeof(T)]; };
+
+__device__ __forceinline__ void widen_four(const raw_four<float> &r, float2 (&v)[2]) {
+  v[0] = make_float2(__uint_as_float(r.w[0]), __uint_as_float(r.w[1]));
+  v[1] = make_float2(__uint_as_float(r.w[2]), __uint_as_float(r.w[3]));
 }
-__device__ __forceinline__ void load_four(const float *x, float *v) {
-  const float4 f = *reinterpret_cast<const float4 *>(x);
-  v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+template <class T> __device__ __forceinline__ void widen_four(const raw_four<T> &r, float2 (&v)[2]) {
+  v[0] = widen_pair(r.w[0], T{}), v[1] = widen_pair(r.w[1], T{});
+}
+
+// column: the lane's first; what is beyond the matrix reads as zero.
+template <bool Vec, class T>
+__device__ __forceinline__ raw_four<T> load_four(const T *row, bool has_row, uint32_t column,
+                                                 uint32_t columns) {
+  raw_four<T> r;
+  if constexpr (Vec) {
+    const bool has = has_row && column < columns;
+    if constexpr (sizeof(T) == 4) {
+      const uint4 u = has ? *reinterpret_cast<const uint4 *>(row + column) : make_uint4(0, 0, 0, 0);
+      r.w[0] = u.x, r.w[1] = u.y, r.w[2] = u.z, r.w[3] = u.w;
+    } else {
+      const uint2 u = has ? *reinterpret_cast<const uint2 *>(row + column) : make_uint2(0, 0);
+      r.w[0] = u.x, r.w[1] = u.y;
+    }
+  } else {
+    using word = typename raw_word<sizeof(T)>::type;
+    const word *x = reinterpret_cast<const word *>(row + column);
+    uint32_t bits[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      bits[j] = has_row && column + 32 * j < columns ? x[32 * j] : word{0};
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)); ++i)
+      r.w[i] = sizeof(T) == 4 ? bits[i] : bits[2 * i % 4] | bits[(2 * i + 1) % 4] << 16;
+  }
+  return r;
 }
 
 template <int Type, int Code, bool Vec>
-__global__ void __launch_bounds__(512) encode_tiles_kernel(const encode_params p) {
+__global__ void __launch_bounds__(tile_of<element_t<Type>>::kThreads,
+                                  1024 / tile_of<element_t<Type>>::kThreads)
+    encode_tiles_kernel(const encode_params p) {
   using T = element_t<Type>;
-  __shared__ float part[16];
+  using tile = tile_of<T>;
+  __shared__ float part[2][tile::kWarps];
   aut::dev::pdl_wait();
   aut::dev::pdl_release();
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
   const uint32_t columns = static_cast<uint32_t>(p.columns);
   const uint32_t blocks = (columns + kBlock - 1) / kBlock;
-  const uint32_t block = blockIdx.x % blocks;
-  const uint64_t group = blockIdx.x / blocks;
-  uint32_t column[4];
+  const uint64_t groups = (p.rows + kBlock - 1) / kBlock;
+  // tile = (row group, column block); blocks take every gridDim.x-th
+  const uint32_t step_groups = gridDim.x / blocks, step_blocks = gridDim.x % blocks;
+  uint64_t group = blockIdx.x / blocks;
+  uint32_t block = blockIdx.x % blocks;
+  const uint32_t lane_column = Vec ? lane * 4 : lane;
+  raw_four<T> next[tile::kRows];
+  auto load = [&] {
+    const uint64_t first = group * kBlock + warp;
+    const T *x = static_cast<const T *>(p.x) + first * p.x_stride;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) column[j] = block * kBlock + (Vec ? lane * 4 + j : lane + 32 * j);
-  float v[8][4], largest = 0.0f;
+    for (int r = 0; r < tile::kRows; ++r)
+      next[r] = load_four<Vec>(x + r * tile::kWarps * p.x_stride,
+                               first + r * tile::kWarps < p.rows, block * kBlock + lane_column,
+                               columns);
+  };
+  load();
+  for (int turn = 0; group < groups; turn ^= 1) {
+    raw_four<T> now[tile::kRows];
 #pragma unroll
-  for (int r = 0; r < 8; ++r) {
-    const uint64_t row = group * kBlock + r * 16 + warp;
-    const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
-    if (Vec && row < p.rows && column[3] < columns) {
-      load_four(x + column[0], v[r]);
-      continue;
+    for (int r = 0; r < tile::kRows; ++r) now[r] = next[r];
+    const uint64_t group_now = group;
+    const uint32_t block_now = block;
+    group += step_groups;
+    block += step_blocks;
+    if (block >= blocks) {
+      block -= blocks;
+      ++group;
     }
+    if (group < groups) load();
+    float largest = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      v[r][j] = row < p.rows && column[j] < columns ? widen(x[column[j]]) : 0.0f;
-  }
-#pragma unroll
-  for (int r = 0; r < 8; ++r)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) largest = fmaxf(largest, finite_magnitude(v[r][j]));
-  largest = warp_max(largest);
-  if (lane == 0) part[warp] = largest;
-  __syncthreads();
-  largest = part[0];
-#pragma unroll
-  for (int w = 1; w < 16; ++w) largest = fmaxf(largest, part[w]);
-  const float scale = scale_of<Code>(largest);
-  const float reciprocal = __frcp_rn(scale);
-  if (threadIdx.x == 0) p.scales[block * p.scale_stride + group] = scale;
-#pragma unroll
-  for (int r = 0; r < 8; ++r) {
-    const uint64_t row = group * kBlock + r * 16 + warp;
-    if (row >= p.rows) break;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[r][j] = quotient(v[r][j], scale, reciprocal);
-    const uint32_t codes = four_codes<Code>(v[r]);
-    uint8_t *to = p.codes + row * p.code_stride;
-    if (Vec && column[3] < columns) {
-      *reinterpret_cast<uint32_t *>(to + column[0]) = codes;
-      continue;
+    for (int r = 0; r < tile::kRows; ++r) {
+      float2 v[2];
+      widen_four(now[r], v);
+      largest = fmaxf(largest, largest_of(v[0], v[1]));
     }
+    largest = warp_max(largest);
+    // two sets of maxima: no warp is more than one tile ahead of another
+    if (lane == 0) part[turn][warp] = largest;
+    __syncthreads();
+    largest = warp_max(part[turn][lane % tile::kWarps]);
+    const bool infinite = largest > 3.40282347e38f; // rare; the same for all
+    if (infinite) {
+      __syncthreads();
+      largest = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (column[j] < columns) to[column[j]] = static_cast<uint8_t>(codes >> (8 * j));
+      for (int r = 0; r < tile::kRows; ++r) {
+        float2 v[2];
+        widen_four(now[r], v);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          largest = fmaxf(largest, fmaxf(finite_magnitude(v[j].x), finite_magnitude(v[j].y)));
+      }
+      largest = warp_max(largest);
+      if (lane == 0) part[turn][warp] = largest;
+      __syncthreads();
+      largest = warp_max(part[turn][lane % tile::kWarps]);
+    }
+    const block_scale s = scale_of<Code>(largest);
+    if (threadIdx.x == 0) p.scales[block_now * p.scale_stride + group_now] = s.scale;
+    const uint64_t first = group_now * kBlock + warp;
+    const uint32_t column = block_now * kBlock + lane_column;
+    uint8_t *to = p.codes + first * p.code_stride + column;
+#pragma unroll
+    for (int r = 0; r < tile::kRows; ++r, to += tile::kWarps * p.code_stride) {
+      float2 v[2];
+      widen_four(now[r], v);
+      if (infinite) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          v[j] = make_float2(without_infinity(v[j].x), without_infinity(v[j].y));
+      }
+      const uint32_t codes = four_codes<Code>(quotient(v[0], s), quotient(v[1], s));
+      const bool has_row = first + r * tile::kWarps < p.rows;
+      if constexpr (Vec) {
+        if (has_row && column < columns) *reinterpret_cast<uint32_t *>(to) = codes;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (has_row && column + 32 * j < columns)
+            to[32 * j] = static_cast<uint8_t>(codes >> (8 * j));
+      }
+    }
   }
 }
 
@@ -275,63 +379,94 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// A row by Threads threads, which hold it in registers (FP32 h, Chunks times
-// eight values a thread), so x and the residual are read once.  Threads = 32:
-// four rows to a block of 128.
+// Rows by Threads threads each, which hold a row in registers (FP32 h, Chunks
+// times eight values a thread), so x and the residual are read once; the
+// weight stays in registers over the rows of a block.  The next row's values
+// are loaded before this one's are summed and encoded.  Threads = 32: four
+// rows to a block of 128.
 template <int Type, int Code, bool Vec, int Threads, int Chunks>
-__global__ void __launch_bounds__(Threads < 128 ? 128 : Threads)
+__global__ void __launch_bounds__(Threads < 128 ? 128 : Threads,
+                                  65536 / (Threads < 512 ? 80 : 64) /
+                                      (Threads < 128 ? 128 : Threads))
     norm_kernel(const norm_params p) {
   using T = element_t<Type>;
   constexpr int kWarps = Threads / 32;
-  __shared__ float part[kWarps];
+  __shared__ float part[2][kWarps];
   aut::dev::pdl_wait();
   aut::dev::pdl_release();
   const int lane = threadIdx.x & 31;
   const int warp = Threads == 32 ? 0 : threadIdx.x / 32;
-  const uint64_t row = Threads == 32 ? uint64_t{blockIdx.x} * 4 + threadIdx.x / 32 : blockIdx.x;
+  const uint64_t rows_a_block = Threads == 32 ? 4 : 1;
+  const uint64_t step = gridDim.x * rows_a_block;
+  uint64_t row = blockIdx.x * rows_a_block + (Threads == 32 ? threadIdx.x / 32 : 0);
   if (row >= p.e.rows) return; // whole warps; whole blocks where a block has one row
   const uint32_t columns = static_cast<uint32_t>(p.e.columns);
+  const float mean_of = static_cast<float>(columns);
   const T *x = static_cast<const T *>(p.e.x) + row * p.e.x_stride;
-  float h[Chunks][8], sum = 0.0f;
+  const T *residual = static_cast<const T *>(p.residual) + row * p.residual_stride;
+  raw_chunk<T> next[Chunks], more[Chunks], weight[Chunks];
 #pragma unroll
-  for (int i = 0; i < Chunks; ++i) load_chunk<Vec>(x, i * kWarps + warp, lane, columns, h[i]);
-  if (p.residual != nullptr) {
-    const T *residual = static_cast<const T *>(p.residual) + row * p.residual_stride;
-#pragma unroll
-    for (int i = 0; i < Chunks; ++i) {
-      float r[8];
-      load_chunk<Vec>(residual, i * kWarps + warp, lane, columns, r);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) h[i][j] += r[j];
-    }
+  for (int i = 0; i < Chunks; ++i) {
+    next[i] = load_raw<Vec>(x, i * kWarps + warp, lane, columns);
+    if (p.residual != nullptr)
+      more[i] = load_raw<Vec>(residual, i * kWarps + warp, lane, columns);
   }
 #pragma unroll
   for (int i = 0; i < Chunks; ++i)
+    if (p.weight != nullptr)
+      weight[i] = load_raw<Vec>(static_cast<const T *>(p.weight), i * kWarps + warp, lane, columns);
+  for (int turn = 0; row < p.e.rows; row += step, turn ^= 1) {
+    float2 h[Chunks][4], squares = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j], h[i][j], sum);
-  sum = warp_sum(sum);
-  if (Threads > 32) {
-    if (lane == 0) part[warp] = sum;
-    __syncthreads();
-    sum = warp_sum(lane < kWarps ? part[lane] : 0.0f);
-  }
-  const float r = rsqrtf(sum / static_cast<float>(columns) + p.eps);
+    for (int i = 0; i < Chunks; ++i) {
+      widen_chunk(next[i], h[i]);
+      if (p.residual != nullptr) {
+        float2 r[4];
+        widen_chunk(more[i], r);
 #pragma unroll
-  for (int i = 0; i < Chunks; ++i) {
-    const uint32_t chunk = i * kWarps + warp;
-    if (chunk * 256 >= columns) break;
-    if (p.residual_out != nullptr)
-      store_chunk<Vec>(static_cast<T *>(p.residual_out) + row * p.residual_stride, chunk, lane,
-                       columns, h[i]);
-    float w[8];
-    if (p.weight != nullptr) load_chunk<Vec>(static_cast<const T *>(p.weight), chunk, lane, columns, w);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      h[i][j] *= r;
-      if (p.weight != nullptr) h[i][j] *= w[j];
+        for (int j = 0; j < 4; ++j) h[i][j] = add2(h[i][j], r[j]);
+      }
     }
-    encode_chunk<Code, Vec>(h[i], chunk, lane, columns, p.e.codes + row * p.e.code_stride,
-                            p.e.scales + row, p.e.scale_stride);
+    if (row + step < p.e.rows) {
+      x += step * p.e.x_stride;
+      residual += step * p.residual_stride;
+#pragma unroll
+      for (int i = 0; i < Chunks; ++i) {
+        next[i] = load_raw<Vec>(x, i * kWarps + warp, lane, columns);
+        if (p.residual != nullptr)
+          more[i] = load_raw<Vec>(residual, i * kWarps + warp, lane, columns);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < Chunks; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) squares = fma2(h[i][j], h[i][j], squares);
+    float sum = warp_sum(squares.x + squares.y);
+    if constexpr (Threads > 32) {
+      // two sets of sums: no warp is more than one row ahead of another
+      if (lane == 0) part[turn][warp] = sum;
+      __syncthreads();
+      sum = warp_sum(lane < kWarps ? part[turn][lane] : 0.0f);
+    }
+    const float r = rsqrtf(sum / mean_of + p.eps);
+#pragma unroll
+    for (int i = 0; i < Chunks; ++i) {
+      const uint32_t chunk = i * kWarps + warp;
+      if (chunk * 256 >= columns) break;
+      if (p.residual_out != nullptr)
+        store_chunk<Vec>(static_cast<T *>(p.residual_out) + row * p.residual_stride, chunk, lane,
+                         columns, h[i]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) h[i][j] = mul2(h[i][j], make_float2(r, r));
+      if (p.weight != nullptr) {
+        float2 w[4];
+        widen_chunk(weight[i], w);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[i][j] = mul2(h[i][j], w[j]);
+      }
+      encode_chunk<Code, Vec>(h[i], chunk, lane, columns, p.e.codes + row * p.e.code_stride,
+                              p.e.scales + row, p.e.scale_stride);
+    }
   }
 }
 
@@ -354,39 +489,39 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const norm_params p) {
                           : static_cast<const T *>(p.residual) + row * p.residual_stride;
   float sum = 0.0f;
   for (uint32_t chunk = warp; chunk < chunks; chunk += 32) {
-    float h[8], s[8];
+    float2 h[4], s[4];
     load_chunk<false>(x, chunk, lane, columns, h);
     if (residual != nullptr) {
       load_chunk<false>(residual, chunk, lane, columns, s);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) h[j] += s[j];
+      for (int j = 0; j < 4; ++j) h[j] = add2(h[j], s[j]);
     }
-    float own = 0.0f;
+    float2 own = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) own = fmaf(h[j], h[j], own);
-    sum += own;
+    for (int j = 0; j < 4; ++j) own = fma2(h[j], h[j], own);
+    sum += own.x + own.y;
   }
   sum = warp_sum(sum);
   if (lane == 0) part[warp] = sum;
   __syncthreads();
   const float r = rsqrtf(warp_sum(part[lane]) / static_cast<float>(columns) + p.eps);
   for (uint32_t chunk = warp; chunk < chunks; chunk += 32) {
-    float h[8], s[8];
+    float2 h[4], s[4];
     load_chunk<false>(x, chunk, lane, columns, h);
     if (residual != nullptr) {
       load_chunk<false>(residual, chunk, lane, columns, s);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) h[j] += s[j];
+      for (int j = 0; j < 4; ++j) h[j] = add2(h[j], s[j]);
     }
     if (p.residual_out != nullptr)
       store_chunk<false>(static_cast<T *>(p.residual_out) + row * p.residual_stride, chunk, lane,
                          columns, h);
-    if (p.weight != nullptr)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = mul2(h[j], make_float2(r, r));
+    if (p.weight != nullptr) {
       load_chunk<false>(static_cast<const T *>(p.weight), chunk, lane, columns, s);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      h[j] *= r;
-      if (p.weight != nullptr) h[j] *= s[j];
+      for (int j = 0; j < 4; ++j) h[j] = mul2(h[j], s[j]);
     }
     encode_chunk<Code, false>(h, chunk, lane, columns, p.e.codes + row * p.e.code_stride,
                               p.e.scales + row, p.e.scale_stride);
@@ -395,11 +530,11 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const norm_params p) {
 
 template <class Params>
 aut_status launch(void (*kernel)(Params), uint64_t grid, int threads, const Params &p,
-                  cudaStream_t stream) {
+                  cudaStream_t stream, unsigned grid_y = 1) {
   if (grid > 0x7fffffffull)
     return aut::lib::fail(AUT_ERR_TOO_LARGE, "more than 2^31 - 1 blocks of rows and columns");
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.gridDim = dim3(static_cast<unsigned>(grid), grid_y);
   cfg.blockDim = dim3(threads);
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
@@ -416,48 +551,87 @@ bool on_boundaries(const void *p, uint64_t rows, uint64_t stride, uint64_t size,
   return reinterpret_cast<uintptr_t>(p) % bytes == 0 && (rows == 1 || stride * size % bytes == 0);
 }
 
+// How many blocks of a kernel run on one SM at a time.
+template <class Params> int resident_blocks(void (*kernel)(Params), int threads) {
+  int n = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) != cudaSuccess) n = 1;
+  return std::max(n, 1);
+}
+
+// All the kernels run as many blocks as fit at one time, each block over many
+// rows or tiles.
+template <int Type, int Code, bool Vec>
+aut_status encode_by_rows(aut_workspace *ws, const encode_params &p, cudaStream_t stream) {
+  auto kernel = encode_rows_kernel<Type, Code, Vec>;
+  static const int resident = resident_blocks(kernel, 256);
+  const uint64_t chunks = (p.columns + 255) / 256;
+  const uint64_t groups = (p.rows + kEncodeRows - 1) / kEncodeRows;
+  const uint64_t most = std::max<uint64_t>(1, static_cast<uint64_t>(resident * ws->sm_count) / chunks);
+  return launch(kernel, chunks, 256, p, stream, static_cast<unsigned>(std::min(groups, most)));
+}
+
+template <int Type, int Code, bool Vec>
+aut_status encode_by_tiles(aut_workspace *ws, const encode_params &p, cudaStream_t stream) {
+  constexpr int kThreads = tile_of<element_t<Type>>::kThreads;
+  auto kernel = encode_tiles_kernel<Type, Code, Vec>;
+  static const int resident = resident_blocks(kernel, kThreads);
+  const uint64_t tiles =
+      (p.rows + kBlock - 1) / kBlock * ((p.columns + kBlock - 1) / kBlock);
+  return launch(kernel, std::min(tiles, static_cast<uint64_t>(resident * ws->sm_count)), kThreads,
+                p, stream);
+}
+
 template <int Type, int Code>
-aut_status encode_typed(int32_t block_rows, const encode_params &p, cudaStream_t stream) {
+aut_status encode_typed(aut_workspace *ws, int32_t block_rows, const encode_params &p,
+                        cudaStream_t stream) {
   constexpr uint64_t size = sizeof(element_t<Type>);
   if (block_rows == 1) {
-    const uint64_t grid = (p.rows + kEncodeRows - 1) / kEncodeRows * ((p.columns + 255) / 256);
-    const bool vec = on_boundaries(p.x, p.rows, p.x_stride, size, 16) &&
+    const bool vec = p.columns % 8 == 0 && on_boundaries(p.x, p.rows, p.x_stride, size, 16) &&
                      on_boundaries(p.codes, p.rows, p.code_stride, 1, 8);
-    return launch(vec ? encode_rows_kernel<Type, Code, true> : encode_rows_kernel<Type, Code, false>,
-                  grid, 256, p, stream);
+    return vec ? encode_by_rows<Type, Code, true>(ws, p, stream)
+               : encode_by_rows<Type, Code, false>(ws, p, stream);
   }
-  const uint64_t grid = (p.rows + kBlock - 1) / kBlock * ((p.columns + kBlock - 1) / kBlock);
-  const bool vec = on_boundaries(p.x, p.rows, p.x_stride, size, 4 * size) &&
+  const bool vec = p.columns % 4 == 0 && on_boundaries(p.x, p.rows, p.x_stride, size, 4 * size) &&
                    on_boundaries(p.codes, p.rows, p.code_stride, 1, 4);
-  return launch(vec ? encode_tiles_kernel<Type, Code, true> : encode_tiles_kernel<Type, Code, false>,
-                grid, 512, p, stream);
+  return vec ? encode_by_tiles<Type, Code, true>(ws, p, stream)
+             : encode_by_tiles<Type, Code, false>(ws, p, stream);
 }
 
-// The fewest threads that hold a row with 16 values each (32 beyond 16384
-// columns, where a block has no more threads).
+template <int Type, int Code, bool Vec, int Threads>
+aut_status norm_launch(aut_workspace *ws, const norm_params &p, cudaStream_t stream) {
+  constexpr int kBlockThreads = Threads < 128 ? 128 : Threads;
+  auto kernel = norm_kernel<Type, Code, Vec, Threads, 2>;
+  static const int resident = resident_blocks(kernel, kBlockThreads);
+  const uint64_t blocks = Threads == 32 ? (p.e.rows + 3) / 4 : p.e.rows;
+  return launch(kernel, std::min(blocks, static_cast<uint64_t>(resident * ws->sm_count)),
+                kBlockThreads, p, stream);
+}
+
+// The fewest threads that hold a row with 16 values each.
 template <int Type, int Code, bool Vec>
-aut_status norm_rows(const norm_params &p, cudaStream_t stream) {
-  const uint64_t rows = p.e.rows, columns = p.e.columns;
-  if (columns <= 512)
-    return launch(norm_kernel<Type, Code, Vec, 32, 2>, (rows + 3) / 4, 128, p, stream);
-  if (columns <= 2048) return launch(norm_kernel<Type, Code, Vec, 128, 2>, rows, 128, p, stream);
-  if (columns <= 8192) return launch(norm_kernel<Type, Code, Vec, 512, 2>, rows, 512, p, stream);
-  return launch(norm_kernel<Type, Code, Vec, 1024, 4>, rows, 1024, p, stream);
+aut_status norm_rows(aut_workspace *ws, const norm_params &p, cudaStream_t stream) {
+  const uint64_t columns = p.e.columns;
+  if (columns <= 512) return norm_launch<Type, Code, Vec, 32>(ws, p, stream);
+  if (columns <= 2048) return norm_launch<Type, Code, Vec, 128>(ws, p, stream);
+  if (columns <= 4096) return norm_launch<Type, Code, Vec, 256>(ws, p, stream);
+  if (columns <= 8192) return norm_launch<Type, Code, Vec, 512>(ws, p, stream);
+  return norm_launch<Type, Code, Vec, 1024>(ws, p, stream);
 }
 
 template <int Type, int Code>
-aut_status norm_typed(const norm_params &p, cudaStream_t stream) {
+aut_status norm_typed(aut_workspace *ws, const norm_params &p, cudaStream_t stream) {
   constexpr uint64_t size = sizeof(element_t<Type>);
-  if (p.e.columns > 32768)
+  if (p.e.columns > 16384)
     return launch(norm_long_kernel<Type, Code>, p.e.rows, 1024, p, stream);
-  const bool vec = on_boundaries(p.e.x, p.e.rows, p.e.x_stride, size, 16) &&
+  const bool vec = p.e.columns % 8 == 0 && on_boundaries(p.e.x, p.e.rows, p.e.x_stride, size, 16) &&
                    (p.residual == nullptr ||
                     on_boundaries(p.residual, p.e.rows, p.residual_stride, size, 16)) &&
                    (p.residual_out == nullptr ||
                     on_boundaries(p.residual_out, p.e.rows, p.residual_stride, size, 16)) &&
                    (p.weight == nullptr || on_boundaries(p.weight, 1, 0, size, 16)) &&
                    on_boundaries(p.e.codes, p.e.rows, p.e.code_stride, 1, 8);
-  return vec ? norm_rows<Type, Code, true>(p, stream) : norm_rows<Type, Code, false>(p, stream);
+  return vec ? norm_rows<Type, Code, true>(ws, p, stream)
+             : norm_rows<Type, Code, false>(ws, p, stream);
 }
 
 } // namespace
@@ -466,7 +640,7 @@ aut_status norm_typed(const norm_params &p, cudaStream_t stream) {
 namespace aut::lib {
 using namespace aut::scaled;
 
-aut_status encode_scaled_launch(aut_workspace *, int32_t code, int32_t type, int32_t block_rows,
+aut_status encode_scaled_launch(aut_workspace *ws, int32_t code, int32_t type, int32_t block_rows,
                                 const void *values, uint64_t rows, uint64_t columns,
                                 uint64_t value_stride, void *codes, uint64_t code_stride,
                                 float *scales, uint64_t scale_stride, cudaStream_t stream) {
@@ -475,18 +649,18 @@ aut_status encode_scaled_launch(aut_workspace *, int32_t code, int32_t type, int
   const bool e4m3 = code == AUT_FP8_E4M3;
   switch (type) {
   case AUT_TYPE_FP32:
-    return e4m3 ? encode_typed<AUT_TYPE_FP32, AUT_FP8_E4M3>(block_rows, p, stream)
-                : encode_typed<AUT_TYPE_FP32, AUT_FP8_E5M2>(block_rows, p, stream);
+    return e4m3 ? encode_typed<AUT_TYPE_FP32, AUT_FP8_E4M3>(ws, block_rows, p, stream)
+                : encode_typed<AUT_TYPE_FP32, AUT_FP8_E5M2>(ws, block_rows, p, stream);
   case AUT_TYPE_BF16:
-    return e4m3 ? encode_typed<AUT_TYPE_BF16, AUT_FP8_E4M3>(block_rows, p, stream)
-                : encode_typed<AUT_TYPE_BF16, AUT_FP8_E5M2>(block_rows, p, stream);
+    return e4m3 ? encode_typed<AUT_TYPE_BF16, AUT_FP8_E4M3>(ws, block_rows, p, stream)
+                : encode_typed<AUT_TYPE_BF16, AUT_FP8_E5M2>(ws, block_rows, p, stream);
   default:
-    return e4m3 ? encode_typed<AUT_TYPE_FP16, AUT_FP8_E4M3>(block_rows, p, stream)
-                : encode_typed<AUT_TYPE_FP16, AUT_FP8_E5M2>(block_rows, p, stream);
+    return e4m3 ? encode_typed<AUT_TYPE_FP16, AUT_FP8_E4M3>(ws, block_rows, p, stream)
+                : encode_typed<AUT_TYPE_FP16, AUT_FP8_E5M2>(ws, block_rows, p, stream);
   }
 }
 
-aut_status rms_norm_scaled_launch(aut_workspace *, int32_t code, int32_t type, const void *x,
+aut_status rms_norm_scaled_launch(aut_workspace *ws, int32_t code, int32_t type, const void *x,
                                   uint64_t x_stride, const void *residual, void *residual_out,
                                   uint64_t residual_stride, const void *weight, float eps,
                                   uint64_t rows, uint64_t columns, void *codes,
@@ -503,14 +677,14 @@ aut_status rms_norm_scaled_launch(aut_workspace *, int32_t code, int32_t type, c
   const bool e4m3 = code == AUT_FP8_E4M3;
   switch (type) {
   case AUT_TYPE_FP32:
-    return e4m3 ? norm_typed<AUT_TYPE_FP32, AUT_FP8_E4M3>(p, stream)
-                : norm_typed<AUT_TYPE_FP32, AUT_FP8_E5M2>(p, stream);
+    return e4m3 ? norm_typed<AUT_TYPE_FP32, AUT_FP8_E4M3>(ws, p, stream)
+                : norm_typed<AUT_TYPE_FP32, AUT_FP8_E5M2>(ws, p, stream);
   case AUT_TYPE_BF16:
-    return e4m3 ? norm_typed<AUT_TYPE_BF16, AUT_FP8_E4M3>(p, stream)
-                : norm_typed<AUT_TYPE_BF16, AUT_FP8_E5M2>(p, stream);
+    return e4m3 ? norm_typed<AUT_TYPE_BF16, AUT_FP8_E4M3>(ws, p, stream)
+                : norm_typed<AUT_TYPE_BF16, AUT_FP8_E5M2>(ws, p, stream);
   default:
-    return e4m3 ? norm_typed<AUT_TYPE_FP16, AUT_FP8_E4M3>(p, stream)
-                : norm_typed<AUT_TYPE_FP16, AUT_FP8_E5M2>(p, stream);
+    return e4m3 ? norm_typed<AUT_TYPE_FP16, AUT_FP8_E4M3>(ws, p, stream)
+                : norm_typed<AUT_TYPE_FP16, AUT_FP8_E5M2>(ws, p, stream);
   }
 }
 

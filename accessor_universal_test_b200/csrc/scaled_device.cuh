@@ -49,24 +49,66 @@ template <int Code> __device__ __forceinline__ uint32_t codes_of(float lo, float
   return r;
 }
 
-// x / scale rounded to FP32, from the block's one reciprocal: Markstein's
-// correction step (the residual x - q * scale is exact in one FMA) makes the
-// product with the rounded reciprocal the correctly rounded quotient, so a
-// value halfway between two codes goes the way of a true division; three
-// operations a value where a division takes about ten.  (Below |x| = 2^-100
-// the residual may underflow; the quotient is then within 2 ulp.)  An
-// infinite x gives inf - inf = NaN, which encodes as NaN.
-__device__ __forceinline__ float quotient(float x, float scale, float reciprocal) {
-  const float q = x * reciprocal;
-  return fmaf(fmaf(-q, scale, x), reciprocal, q);
+// Two FP32 values in one register pair: one instruction for both.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
 }
 
-// The scale of a block whose largest finite magnitude is `largest`: at least
-// 2^-126, so that its reciprocal is finite and a block of zeros needs no case
-// of its own.
-template <int Code> __device__ __forceinline__ float scale_of(float largest) {
+// The scale of a block and its reciprocal as the sum of two FP32 values.
+struct block_scale {
+  float scale, inverse, rest;
+};
+
+// From the block's largest finite magnitude.  The scale, largest / F rounded
+// once, is at least 2^-126: its reciprocal is then finite and a block of zeros
+// needs no case of its own.  The division by the constant F is a product with
+// 1 / F and Markstein's correction (the residual is exact in one FMA).  The
+// reciprocal starts from the hardware's approximation r; with e = 1 - scale r,
+// exact in one FMA, 1 / scale = r + r (e + e^2) up to r e^3.
+template <int Code> __device__ __forceinline__ block_scale scale_of(float largest) {
   constexpr float f = largest_code<Code>(), reciprocal = 1.0f / f;
-  return fmaxf(quotient(largest, f, reciprocal), 1.17549435e-38f);
+  block_scale s;
+  const float q = largest * reciprocal;
+  s.scale = fmaxf(fmaf(fmaf(-q, f, largest), reciprocal, q), 1.17549435e-38f);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.inverse) : "f"(s.scale));
+  const float e = fmaf(-s.scale, s.inverse, 1.0f);
+  s.rest = s.inverse * fmaf(e, e, e);
+  return s;
+}
+
+// x / scale for two values, finite or NaN.  x * inverse + x * rest is within
+// 2^-44 of the quotient before its one rounding to FP32, so the codes are
+// those of a correctly rounded division, ties included: a quotient of two
+// FP32 values is a tie between codes exactly or at least 2^-29 away from it.
+// Two operations for two values, where a division takes about ten for each.
+// (For scales above 2^100 the rest loses digits: the quotient is then within
+// 2 ulp.)
+__device__ __forceinline__ float2 quotient(float2 x, const block_scale &s) {
+  return fma2(x, make_float2(s.inverse, s.inverse), mul2(x, make_float2(s.rest, s.rest)));
 }
 
 // |v| for a block's largest magnitude: infinities and NaN do not count.
@@ -75,10 +117,17 @@ __device__ __forceinline__ float finite_magnitude(float v) {
   return a <= 3.40282347e38f ? a : 0.0f;
 }
 
+// Largest over the warp of values that are not negative, NaN passed over: their
+// bit patterns order as integers.
 __device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-  return v;
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(v, 0.0f))));
+}
+
+// The same over each half of the warp: two reductions of the whole warp, since
+// a reduction under two masks would part the halves' ways.
+__device__ __forceinline__ float half_warp_max(float v, int lane) {
+  const float low = warp_max(lane < 16 ? v : 0.0f), high = warp_max(lane < 16 ? 0.0f : v);
+  return lane < 16 ? low : high;
 }
 
 } // namespace aut::scaled
