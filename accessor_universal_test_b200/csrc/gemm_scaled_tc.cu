@@ -5,18 +5,34 @@
 // b_scale[b, column / 128].  The scales are FP32, so they cannot go into the
 // instruction: each block's product is made in tensor memory by itself (four
 // instructions of 32 codes, the first without an addend) and added, times its
-// scales, to the sums in the epilogue warps' registers, while the next block's
-// product is made in the other half of tensor memory.
+// scales, to the sums in the epilogue warps' registers, while the next blocks'
+// products are made elsewhere in tensor memory.
+//
+// Roles: warps 0-7 scale and add and, at the end of a tile, store; of the
+// last warpgroup, one warp loads the operands' tiles, one issues the products
+// and two bring the scales.
 #include "gemm_scaled.cuh"
 
 #include <cuda.h>
 
+#include <algorithm>
+#include <atomic>
+
 namespace aut::scaled {
 namespace {
 
+constexpr int kMaxDevices = 16;
 constexpr int kTileM = 128;
 constexpr int kEpilogueWarps = 8;
-constexpr int kTileThreads = 32 * (kEpilogueWarps + 2);
+constexpr int kLoadWarp = kEpilogueWarps, kProductWarp = kEpilogueWarps + 1,
+              kScaleWarp = kEpilogueWarps + 2; // and the next, one for each side
+constexpr int kTileThreads = 32 * (kEpilogueWarps + 4);
+// Blocks of k whose scales are brought at a time, and how many such batches
+// there is room for.
+constexpr int kScaleBatch = 4, kScaleSlots = 4;
+// A load takes a few thousand cycles at most: a pair's pause for them once one
+// of its waits has given up (about half a millisecond).
+constexpr long long kPairDrainCycles = 1000000;
 
 struct tile_params {
   gemm_params g;
@@ -71,34 +87,114 @@ __device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, long lo
   }
 }
 
-__device__ __forceinline__ void load_tile(void *dst, const CUtensorMap *map, int column, int row,
-                                          uint64_t *bar) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-               "[%0], [%1, {%2, %3}], [%4];" ::"r"(smem_addr(dst)),
-               "l"(map), "r"(column), "r"(row), "r"(smem_addr(bar))
+// Address, in the pair's shared memory, of what stands at `p` in its first block.
+__device__ __forceinline__ uint32_t leader_addr(const void *p) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_addr(p)));
+  return a;
+}
+
+// Arrives on a barrier of the pair's first block.  Relaxed: what the arrival
+// hands over is tensor memory that has been read (tcgen05.wait::ld and the
+// fence before it order that); a release over the cluster waits for all of the
+// thread's memory operations, about a thousand cycles.
+__device__ __forceinline__ void bar_arrive_leader(uint64_t *bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                   leader_addr(bar))
                : "memory");
+}
+
+__device__ __forceinline__ void pair_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\t"
+               "barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// The loads of both blocks of a pair are counted on its first block's barrier.
+template <bool Pair>
+__device__ __forceinline__ void load_tile(void *dst, const CUtensorMap *map, int column, int row,
+                                          uint32_t bar) {
+  if constexpr (Pair)
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile"
+                 ".mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_addr(dst)),
+                 "l"(map), "r"(column), "r"(row), "r"(bar)
+                 : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile"
+                 ".mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_addr(dst)),
+                 "l"(map), "r"(column), "r"(row), "r"(bar)
+                 : "memory");
 }
 
 // Shared-memory descriptor of a tile of rows of 128 bytes with the 128-byte
-// swizzle: eight rows make an atom of 1024 bytes, the stride between atoms.
-__device__ __forceinline__ uint64_t tile_descriptor(uint32_t addr) {
-  return static_cast<uint64_t>((addr & 0x3ffffu) >> 4) | (uint64_t{1} << 16) |
-         (uint64_t{1024 >> 4} << 32) | (uint64_t{1} << 46) | (uint64_t{2} << 61);
+// swizzle (eight rows make an atom of 1024 bytes, the stride between atoms): the
+// low word holds the address in units of 16 bytes, the high word is constant.
+__device__ __forceinline__ uint32_t descriptor_low(uint32_t addr) {
+  return ((addr & 0x3ffffu) >> 4) | 1u << 16;
+}
+constexpr uint32_t kDescriptorHigh = (1024 >> 4) | 1u << 14 | 2u << 29;
+
+// One thread issues all products, so it must not compute between them: the
+// descriptors differ by a constant in the low word, and whether the product is
+// added is known at compile time.
+template <bool Pair, bool Add>
+__device__ __forceinline__ void mma_f8(uint32_t tmem, uint32_t a, uint32_t b, uint32_t idesc) {
+#define AUT_MMA_F8(group)                                                                  \
+  asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"                                 \
+               "setp.ne.b32 p, %4, 0;\n\t"                                                 \
+               "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"                          \
+               "tcgen05.mma.cta_group::" group ".kind::f8f6f4 [%0], a, b, %3, p;\n\t}" ::   \
+                   "r"(tmem),                                                              \
+               "r"(a), "r"(b), "r"(idesc), "n"(Add ? 1 : 0), "r"(kDescriptorHigh)          \
+               : "memory")
+  if constexpr (Pair) AUT_MMA_F8("2");
+  else AUT_MMA_F8("1");
+#undef AUT_MMA_F8
 }
 
-__device__ __forceinline__ void mma_f8(uint32_t tmem, uint64_t a, uint64_t b, uint32_t idesc,
-                                       bool add) {
-  asm volatile("{\n\t.reg .pred p;\n\t"
-               "setp.ne.b32 p, %4, 0;\n\t"
-               "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
-               "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
-               : "memory");
+// The product of a block of 128 codes: four instructions of 32.
+template <bool Pair>
+__device__ __forceinline__ void mma_block(uint32_t tmem, uint32_t a, uint32_t b, uint32_t idesc) {
+  mma_f8<Pair, false>(tmem, a, b, idesc);
+  mma_f8<Pair, true>(tmem, a + 2, b + 2, idesc);
+  mma_f8<Pair, true>(tmem, a + 4, b + 4, idesc);
+  mma_f8<Pair, true>(tmem, a + 6, b + 6, idesc);
 }
 
-__device__ __forceinline__ void mma_commit(uint64_t *bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   smem_addr(bar))
-               : "memory");
+// Arrives on the barrier, of both blocks where it is a pair, once the
+// instructions issued so far are done.
+template <bool Pair> __device__ __forceinline__ void mma_commit(uint64_t *bar) {
+  if constexpr (Pair)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster"
+                 ".multicast::cluster.b64 [%0], %1;" ::"r"(smem_addr(bar)),
+                 "h"(static_cast<uint16_t>(3))
+                 : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::
+                     "r"(smem_addr(bar))
+                 : "memory");
+}
+
+template <bool Pair, int Columns> __device__ __forceinline__ void tmem_alloc(uint32_t *base) {
+  if constexpr (Pair) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_addr(base)),
+                 "n"(Columns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_addr(base)),
+                 "n"(Columns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+}
+
+template <bool Pair, int Columns> __device__ __forceinline__ void tmem_free(uint32_t base) {
+  if constexpr (Pair)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "n"(Columns));
+  else
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "n"(Columns));
 }
 
 // 32 lanes x W columns of tensor memory; the values are there after
@@ -144,44 +240,59 @@ __device__ __forceinline__ uint32_t pack_fp16(float lo, float hi) {
 
 // Eight neighbouring results of row i from column j on.
 __device__ __forceinline__ void store_eight(const tile_params &p, uint64_t i, uint64_t j,
-                                            const float *v) {
+                                            const float2 *v) {
   const gemm_params &g = p.g;
   if (p.wide_out && j + 8 <= g.n) {
     const uint64_t at = i * g.out_stride + j;
     if (g.type == AUT_TYPE_FP32) {
       float4 *o = reinterpret_cast<float4 *>(static_cast<float *>(g.out) + at);
-      o[0] = make_float4(v[0], v[1], v[2], v[3]);
-      o[1] = make_float4(v[4], v[5], v[6], v[7]);
+      o[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+      o[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
     } else if (g.type == AUT_TYPE_BF16) {
       *reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(g.out) + at) =
-          make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]),
-                     pack_bf16(v[6], v[7]));
+          make_uint4(pack_bf16(v[0].x, v[0].y), pack_bf16(v[1].x, v[1].y),
+                     pack_bf16(v[2].x, v[2].y), pack_bf16(v[3].x, v[3].y));
     } else {
       *reinterpret_cast<uint4 *>(static_cast<__half *>(g.out) + at) =
-          make_uint4(pack_fp16(v[0], v[1]), pack_fp16(v[2], v[3]), pack_fp16(v[4], v[5]),
-                     pack_fp16(v[6], v[7]));
+          make_uint4(pack_fp16(v[0].x, v[0].y), pack_fp16(v[1].x, v[1].y),
+                     pack_fp16(v[2].x, v[2].y), pack_fp16(v[3].x, v[3].y));
     }
     return;
   }
 #pragma unroll
-  for (int c = 0; c < 8; ++c)
-    if (j + c < g.n) store_out(g, i, j + c, v[c]);
+  for (int c = 0; c < 4; ++c) {
+    if (j + 2 * c < g.n) store_out(g, i, j + 2 * c, v[c].x);
+    if (j + 2 * c + 1 < g.n) store_out(g, i, j + 2 * c + 1, v[c].y);
+  }
 }
 
-template <int BN> struct tile_shape {
+// BN columns of out by 128 rows for each block; the two blocks of a pair share
+// the columns, and each holds half of the rows of b that they stand for.
+// Tensor memory holds the products of kDepth blocks of k.  With 256 columns
+// that is two, too few to hide the way from the products to the epilogue and
+// back; there each side of the columns is a unit of its own, made, read and
+// given back by itself.
+template <int BN, bool Pair> struct tile_shape {
   static constexpr int kABytes = kTileM * kBlock;
-  static constexpr int kBBytes = BN * kBlock;
+  static constexpr int kBRows = Pair ? BN / 2 : BN;
+  static constexpr int kBBytes = kBRows * kBlock;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = 200 * 1024 / kStageBytes < 8 ? 200 * 1024 / kStageBytes : 8;
+  static constexpr int kStages = 192 * 1024 / kStageBytes < 8 ? 192 * 1024 / kStageBytes : 8;
   static constexpr int kSmem = kStages * kStageBytes + 1024;
-  static constexpr int kTmemColumns = 2 * BN;
+  static constexpr int kDepth = BN == 256 ? 2 : 4;
+  static constexpr int kSides = 1; // units of a block of k
+  static constexpr int kUnits = kDepth * kSides;
+  static constexpr int kUnitColumns = BN / kSides;
+  static constexpr int kTmemColumns = kDepth * BN;
+  static constexpr int kTileRows = Pair ? 2 * kTileM : kTileM; // of out, by both blocks
 };
 
-// Tiles in bands of 16 rows of tiles, column by column within a band: the
-// tiles that run at one time share few rows and few columns.
+// Tiles in bands of rows of tiles (2048 rows of a), column by column within a
+// band: the tiles that run at one time share few rows and few columns.
+template <int Rows>
 __device__ __forceinline__ void tile_at(uint32_t tile, const tile_params &p, uint32_t &tm,
                                         uint32_t &tn) {
-  constexpr uint32_t kBand = 16;
+  constexpr uint32_t kBand = 2048 / Rows;
   const uint32_t per_band = kBand * p.tiles_n;
   const uint32_t band = tile / per_band, rest = tile % per_band;
   const uint32_t left = p.tiles_m - band * kBand;
@@ -190,43 +301,52 @@ __device__ __forceinline__ void tile_at(uint32_t tile, const tile_params &p, uin
   tn = rest / height;
 }
 
-template <int BN>
+template <int BN, bool Pair>
 __global__ void __launch_bounds__(kTileThreads, 1)
     tiles_kernel(const __grid_constant__ CUtensorMap map_a,
                  const __grid_constant__ CUtensorMap map_b, const tile_params p) {
-  using shape = tile_shape<BN>;
+  using shape = tile_shape<BN, Pair>;
   constexpr int kStages = shape::kStages;
   extern __shared__ unsigned char dynamic[];
   unsigned char *ring = reinterpret_cast<unsigned char *>(
       (reinterpret_cast<uintptr_t>(dynamic) + 1023) & ~uintptr_t{1023});
-  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], made[2], taken[2], drained;
+  __shared__ __align__(8) uint64_t full[kStages], empty[kStages];
+  __shared__ __align__(8) uint64_t made[shape::kUnits], taken[shape::kUnits];
+  __shared__ __align__(8) uint64_t scales_in[2][kScaleSlots], scales_used[2][kScaleSlots];
+  __shared__ __align__(8) uint64_t drained;
+  __shared__ float scales[2][kScaleSlots][kScaleBatch][kTileM]; // of both operands, by sides
   __shared__ uint32_t tmem_base;
   __shared__ int gave_up_word;
   volatile int *gave_up = &gave_up_word;
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const uint32_t rank = Pair ? blockIdx.x % 2 : 0;
+  const uint32_t worker = Pair ? blockIdx.x / 2 : blockIdx.x;
+  const uint32_t workers = Pair ? gridDim.x / 2 : gridDim.x;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       bar_init(&full[s], 1);
       bar_init(&empty[s], 1);
     }
-    for (int s = 0; s < 2; ++s) {
-      bar_init(&made[s], 1);
-      bar_init(&taken[s], kEpilogueWarps);
+    for (int u = 0; u < shape::kUnits; ++u) {
+      bar_init(&made[u], 1);
+      bar_init(&taken[u], (Pair ? 2 : 1) * kEpilogueWarps / shape::kSides);
     }
+    for (int side = 0; side < 2; ++side)
+      for (int s = 0; s < kScaleSlots; ++s) {
+        bar_init(&scales_in[side][s], 1);
+        bar_init(&scales_used[side][s], kEpilogueWarps / 2);
+      }
     bar_init(&drained, 1);
     gave_up_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == kEpilogueWarps + 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     smem_addr(&tmem_base)),
-                 "n"(shape::kTmemColumns)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  if (warp == kProductWarp) {
+    tmem_alloc<Pair, shape::kTmemColumns>(&tmem_base);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   }
   __syncthreads();
+  if (Pair) pair_sync(); // the barriers of both blocks are there
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmem_base;
 
@@ -236,135 +356,212 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const uint32_t tiles = p.tiles_m * p.tiles_n;
   const uint32_t blocks = static_cast<uint32_t>((p.g.k + kBlock - 1) / kBlock);
   uint64_t loads = 0; // by the loading thread
-  if (warp == kEpilogueWarps) {
-    if (lane == 0) {
-      for (uint32_t tile = blockIdx.x; tile < tiles && *gave_up == 0; tile += gridDim.x) {
+  if (warp >= kEpilogueWarps) {
+    // 12 warps were launched with 168 registers a thread: 8 x 200 + 4 x 104
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if (warp == kLoadWarp && lane == 0) {
+      int s = 0;
+      uint32_t parity = 1; // of the wait for a free stage; at first all are
+      for (uint32_t tile = worker; tile < tiles && *gave_up == 0; tile += workers) {
         uint32_t tm, tn;
-        tile_at(tile, p, tm, tn);
+        tile_at<shape::kTileRows>(tile, p, tm, tn);
+        const int a_row = static_cast<int>(tm * shape::kTileRows + rank * kTileM);
+        const int b_row =
+            static_cast<int>(tn * BN + rank * (shape::kBRows / shape::kSides));
         for (uint32_t block = 0; block < blocks; ++block) {
-          const int s = static_cast<int>(loads % kStages);
-          if (loads >= kStages &&
-              !bar_wait(&empty[s], static_cast<uint32_t>(loads / kStages - 1) & 1u, p.wait_cycles,
-                        gave_up)) {
+          if (!bar_wait(&empty[s], parity, p.wait_cycles, gave_up)) {
             *gave_up = 1;
             break;
           }
           unsigned char *stage = ring + s * shape::kStageBytes;
-          bar_expect(&full[s], shape::kStageBytes);
+          if (rank == 0) bar_expect(&full[s], (Pair ? 2 : 1) * shape::kStageBytes);
+          const uint32_t bar = Pair ? leader_addr(&full[s]) : smem_addr(&full[s]);
           if (loads != p.stall_tile) {
-            load_tile(stage, &map_a, static_cast<int>(block * kBlock),
-                      static_cast<int>(tm * kTileM), &full[s]);
-            load_tile(stage + shape::kABytes, &map_b, static_cast<int>(block * kBlock),
-                      static_cast<int>(tn * BN), &full[s]);
+            const int column = static_cast<int>(block * kBlock);
+            load_tile<Pair>(stage, &map_a, column, a_row, bar);
+#pragma unroll
+            for (int side = 0; side < shape::kSides; ++side)
+              load_tile<Pair>(stage + shape::kABytes + side * (shape::kBBytes / shape::kSides),
+                              &map_b, column, b_row + side * shape::kUnitColumns, bar);
           }
           ++loads;
+          if (++s == kStages) s = 0, parity ^= 1;
         }
       }
     }
-  } else if (warp == kEpilogueWarps + 1) {
-    if (lane == 0) {
-      uint64_t step = 0;
-      for (uint32_t tile = blockIdx.x; tile < tiles && *gave_up == 0; tile += gridDim.x) {
-        for (uint32_t block = 0; block < blocks; ++block, ++step) {
-          const int s = static_cast<int>(step % kStages), half = static_cast<int>(step & 1);
-          if ((step >= 2 && !bar_wait(&taken[half], static_cast<uint32_t>(step / 2 - 1) & 1u,
-                                      p.wait_cycles, gave_up)) ||
-              !bar_wait(&full[s], static_cast<uint32_t>(step / kStages) & 1u, p.wait_cycles,
-                        gave_up)) {
+    if (warp == kProductWarp && lane == 0 && rank == 0) {
+      const uint32_t a0 = descriptor_low(smem_addr(ring));
+      int s = 0, depth = 0;
+      uint32_t parity = 0, free_parity = 1; // tensor memory is all free at first
+      for (uint32_t tile = worker; tile < tiles && *gave_up == 0; tile += workers) {
+        for (uint32_t block = 0; block < blocks; ++block) {
+          const uint32_t a = a0 + s * (shape::kStageBytes >> 4);
+          bool ok = bar_wait(&full[s], parity, p.wait_cycles, gave_up);
+#pragma unroll
+          for (int side = 0; side < shape::kSides; ++side) {
+            const int u = depth * shape::kSides + side;
+            ok = ok && bar_wait(&taken[u], free_parity, p.wait_cycles, gave_up);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            mma_block<Pair>(
+                tmem + u * shape::kUnitColumns, a,
+                a + ((shape::kABytes + side * (shape::kBBytes / shape::kSides)) >> 4), p.idesc);
+            mma_commit<Pair>(&made[u]);
+          }
+          if (!ok) {
             *gave_up = 1;
             break;
           }
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t stage = smem_addr(ring + s * shape::kStageBytes);
+          mma_commit<Pair>(&empty[s]);
+          if (++s == kStages) s = 0, parity ^= 1;
+          if (++depth == shape::kDepth) depth = 0, free_parity ^= 1;
+        }
+      }
+    }
+    if (warp >= kScaleWarp) {
+      // a_scale * b_scale of 128 rows and one side of the columns, four rows a
+      // lane, a batch of blocks at a time
+      const int side = warp - kScaleWarp;
+      uint64_t batch = 0;
+      bool ok = true;
+      for (uint32_t tile = worker; tile < tiles && ok; tile += workers) {
+        uint32_t tm, tn;
+        tile_at<shape::kTileRows>(tile, p, tm, tn);
+        const uint64_t i = uint64_t{tm} * shape::kTileRows + rank * kTileM + lane;
+        const uint64_t j = uint64_t{tn} * BN + side * (BN / 2);
+        const float *sa = p.g.a_scales + i;
+        const float *sb = p.g.b_scales + (j < p.g.n ? j / kBlock : 0);
+        for (uint32_t block = 0; block < blocks; block += kScaleBatch, ++batch) {
+          float row[kScaleBatch][4], column[kScaleBatch];
 #pragma unroll
-          for (int i = 0; i < kBlock / 32; ++i)
-            mma_f8(tmem + half * BN, tile_descriptor(stage + 32 * i),
-                   tile_descriptor(stage + shape::kABytes + 32 * i), p.idesc, i > 0);
-          mma_commit(&empty[s]);
-          mma_commit(&made[half]);
+          for (int b = 0; b < kScaleBatch; ++b) {
+            const bool has = block + b < blocks;
+            column[b] = has ? __ldg(sb) : 0.0f;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              row[b][r] = has && i + 32 * r < p.g.m ? __ldg(sa + 32 * r) : 0.0f;
+            sa += p.g.a_scale_stride;
+            sb += p.g.b_scale_stride;
+          }
+          const int slot = static_cast<int>(batch % kScaleSlots);
+          ok = batch < kScaleSlots ||
+               bar_wait(&scales_used[side][slot],
+                        static_cast<uint32_t>(batch / kScaleSlots - 1) & 1u, p.wait_cycles, gave_up);
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            *gave_up = 1;
+            break;
+          }
+#pragma unroll
+          for (int b = 0; b < kScaleBatch; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              scales[side][slot][b][32 * r + lane] = row[b][r] * column[b];
+          __syncwarp();
+          if (lane == 0) bar_arrive(&scales_in[side][slot]);
         }
       }
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // Warps w and w + 4 take the tensor-memory lanes (rows of the tile)
-    // 32 (w % 4) ..., each one half of the columns.
+    // 32 (w % 4) ..., each one side of the columns.
     constexpr int kColumns = BN / 2;
-    constexpr int kChunk = BN == 256 || BN == 32 ? 16 : 32; // 256: registers
+    constexpr int kChunk = kColumns < 32 ? kColumns : 32;
+    constexpr int kChunks = kColumns / kChunk;
     const int row = warp % 4 * 32 + lane, side = warp / 4;
-    const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
-    uint64_t step = 0;
+    const uint32_t tmem_own = tmem + (static_cast<uint32_t>(warp % 4 * 32) << 16) + side * kColumns;
+    uint32_t step = 0, batch = 0;
     bool lost = false;
-    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    for (uint32_t tile = worker; tile < tiles; tile += workers) {
       uint32_t tm, tn;
-      tile_at(tile, p, tm, tn);
-      const uint64_t i = uint64_t{tm} * kTileM + row;
-      const uint64_t j0 = uint64_t{tn} * BN + side * kColumns;
-      const bool has_row = i < p.g.m;
-      const float *sa = p.g.a_scales + i;
-      const float *sb = p.g.b_scales + (j0 < p.g.n ? j0 : 0) / kBlock;
-      float acc[kColumns];
+      tile_at<shape::kTileRows>(tile, p, tm, tn);
+      float2 acc[kColumns / 2];
 #pragma unroll
-      for (int c = 0; c < kColumns; ++c) acc[c] = 0.0f;
-      for (uint32_t block = 0; block < blocks && !lost; ++block, ++step) {
-        const float s = (has_row ? __ldg(sa + block * p.g.a_scale_stride) : 0.0f) *
-                        __ldg(sb + block * p.g.b_scale_stride);
-        const int half = static_cast<int>(step & 1);
-        const bool ok =
-            bar_wait(&made[half], static_cast<uint32_t>(step / 2) & 1u, p.wait_cycles, gave_up);
+      for (int c = 0; c < kColumns / 2; ++c) acc[c] = make_float2(0.0f, 0.0f);
+      for (uint32_t block = 0; block < blocks; ++block, ++step) {
+        const uint32_t at = block % kScaleBatch, slot = batch % kScaleSlots;
+        const uint32_t depth = step % shape::kDepth;
+        const uint32_t u = shape::kSides == 2 ? depth * 2 + side : depth;
+        bool ok = at != 0 || bar_wait(&scales_in[side][slot], batch / kScaleSlots & 1u,
+                                      p.wait_cycles, gave_up);
+        const float s = scales[side][slot][at][row];
+        ok = ok && bar_wait(&made[u], step / shape::kDepth & 1u, p.wait_cycles, gave_up);
         if (!__all_sync(0xffffffffu, ok)) {
           lost = true;
           break;
         }
+        if (at == kScaleBatch - 1 || block + 1 == blocks) {
+          if (lane == 0) bar_arrive(&scales_used[side][slot]);
+          ++batch;
+        }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        float v[2][kChunk];
+        tmem_load(v[0], tmem_own + depth * BN);
 #pragma unroll
-        for (int c0 = 0; c0 < kColumns; c0 += kChunk) {
-          float v[kChunk];
-          __syncwarp();
-          tmem_load(v, tmem + lanes + half * BN + side * kColumns + c0);
-          tmem_wait(v);
-          if (c0 + kChunk == kColumns) {
+        for (int c0 = 0; c0 < kChunks; ++c0) {
+          float(&now)[kChunk] = v[c0 % 2];
+          tmem_wait(now);
+          if (c0 + 1 < kChunks) {
+            tmem_load(v[(c0 + 1) % 2], tmem_own + depth * BN + (c0 + 1) * kChunk);
+          } else {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) bar_arrive(&taken[half]);
+            if (lane == 0) {
+              if (Pair) bar_arrive_leader(&taken[u]);
+              else bar_arrive(&taken[u]);
+            }
           }
 #pragma unroll
-          for (int c = 0; c < kChunk; ++c) acc[c0 + c] = fmaf(v[c], s, acc[c0 + c]);
+          for (int c = 0; c < kChunk / 2; ++c)
+            acc[c0 * kChunk / 2 + c] = fma2(make_float2(now[2 * c], now[2 * c + 1]),
+                                            make_float2(s, s), acc[c0 * kChunk / 2 + c]);
         }
       }
       if (lost) {
         *gave_up = 1;
 #pragma unroll
-        for (int c = 0; c < kColumns; ++c) acc[c] = __int_as_float(0x7fffffff);
+        for (int c = 0; c < kColumns / 2; ++c)
+          acc[c] = make_float2(__int_as_float(0x7fffffff), __int_as_float(0x7fffffff));
       }
-      if (has_row) {
+      const uint64_t i = uint64_t{tm} * shape::kTileRows + rank * kTileM + row;
+      const uint64_t j0 = uint64_t{tn} * BN + side * kColumns;
+      if (i < p.g.m) {
 #pragma unroll
-        for (int c = 0; c < kColumns; c += 8) store_eight(p, i, j0 + c, acc + c);
+        for (int c = 0; c < kColumns; c += 8) store_eight(p, i, j0 + c, acc + c / 2);
       }
     }
   }
   __syncthreads();
   if (*gave_up != 0) {
-    // Let what is under way end before its memory is given back.
-    if (warp == kEpilogueWarps && lane == 0) {
+    // Let what is under way end before its memory is given back: this block's
+    // loads, which in a pair only the first block's barriers show, and the
+    // products.
+    int none = 0;
+    if (warp == kLoadWarp && lane == 0) {
       atomicOr(p.status, static_cast<unsigned int>(AUT_STATUS_WAIT_TIMEOUT));
-      const uint64_t first = loads > kStages ? loads - kStages : 0;
-      int none = 0;
-      for (uint64_t l = first; l < loads; ++l)
-        if (l != p.stall_tile)
-          bar_wait(&full[l % kStages], static_cast<uint32_t>(l / kStages) & 1u, p.wait_cycles,
-                   &none);
+      if (Pair) {
+        const long long start = clock64();
+        while (clock64() - start < kPairDrainCycles) {
+        }
+      } else {
+        for (uint64_t l = loads > kStages ? loads - kStages : 0; l < loads; ++l)
+          if (l != p.stall_tile)
+            bar_wait(&full[l % kStages], static_cast<uint32_t>(l / kStages) & 1u, p.wait_cycles,
+                     &none);
+      }
     }
-    if (warp == kEpilogueWarps + 1 && lane == 0) {
-      int none = 0;
-      mma_commit(&drained);
+    if (warp == kProductWarp && lane == 0 && rank == 0) {
+      mma_commit<Pair>(&drained);
       bar_wait(&drained, 0, p.wait_cycles, &none);
     }
     __syncthreads();
   }
-  if (warp == kEpilogueWarps + 1) {
+  // no block of a pair leaves before the other is done with its barriers
+  if (Pair) pair_sync();
+  if (warp == kProductWarp) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
-                 "n"(shape::kTmemColumns));
+    tmem_free<Pair, shape::kTmemColumns>(tmem);
   }
 }
 
@@ -406,37 +603,59 @@ aut_status make_map(CUtensorMap *map, const uint8_t *codes, uint64_t rows, uint6
   return AUT_OK;
 }
 
-template <int BN>
+template <int BN, bool Pair>
 aut_status launch_tiles(aut_workspace *ws, tile_params p, int a_code, int b_code,
                         cudaStream_t stream) {
-  using shape = tile_shape<BN>;
+  using shape = tile_shape<BN, Pair>;
+  auto kernel = tiles_kernel<BN, Pair>;
   CUtensorMap map_a, map_b;
   aut_status st = make_map(&map_a, p.g.a, p.g.m, p.g.k, p.g.a_stride, kTileM);
-  if (st == AUT_OK) st = make_map(&map_b, p.g.b, p.g.n, p.g.k, p.g.b_stride, BN);
+  if (st == AUT_OK) st = make_map(&map_b, p.g.b, p.g.n, p.g.k, p.g.b_stride,
+                                  shape::kBRows / shape::kSides);
   if (st != AUT_OK) return st;
-  p.tiles_m = static_cast<uint32_t>((p.g.m + kTileM - 1) / kTileM);
-  p.tiles_n = static_cast<uint32_t>((p.g.n + BN - 1) / BN);
-  // FP32 sums, both operands with k contiguous, tiles of 128 x BN
-  p.idesc = (1u << 4) | (static_cast<uint32_t>(a_code) << 7) |
-            (static_cast<uint32_t>(b_code) << 10) | (static_cast<uint32_t>(BN / 8) << 17) |
-            (static_cast<uint32_t>(kTileM / 16) << 24);
-  const uint64_t tiles = uint64_t{p.tiles_m} * p.tiles_n;
-  if (tiles > 0x7fffffffull)
+  const uint64_t tiles_m = (p.g.m + shape::kTileRows - 1) / shape::kTileRows;
+  const uint64_t tiles_n = (p.g.n + BN - 1) / BN;
+  if (tiles_m * tiles_n > 0x7fffffffull)
     return aut::lib::fail(AUT_ERR_TOO_LARGE, "more than 2^31 - 1 tiles of the product");
-  AUT_CUDA_TRY(cudaFuncSetAttribute(tiles_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    shape::kSmem));
+  p.tiles_m = static_cast<uint32_t>(tiles_m);
+  p.tiles_n = static_cast<uint32_t>(tiles_n);
+  // FP32 sums, both operands with k contiguous, units of kTileRows x kUnitColumns
+  p.idesc = (1u << 4) | (static_cast<uint32_t>(a_code) << 7) |
+            (static_cast<uint32_t>(b_code) << 10) | (static_cast<uint32_t>(shape::kUnitColumns / 8) << 17) |
+            (static_cast<uint32_t>(shape::kTileRows / 16) << 24);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(
-      tiles < static_cast<uint64_t>(ws->sm_count) ? tiles : ws->sm_count));
   cfg.blockDim = dim3(kTileThreads);
   cfg.dynamicSmemBytes = shape::kSmem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  AUT_CUDA_TRY(cudaLaunchKernelEx(&cfg, tiles_kernel<BN>, map_a, map_b, p));
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = Pair ? 2 : 1;
+  // once per device and kernel: shared memory, and how many workers run at a time
+  static std::atomic<int> resident[kMaxDevices];
+  int at_once = ws->device < kMaxDevices ? resident[ws->device].load() : 0;
+  if (at_once == 0) {
+    AUT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      shape::kSmem));
+    at_once = ws->sm_count;
+    if (Pair) {
+      cfg.gridDim = dim3(static_cast<unsigned>(ws->sm_count / 2 * 2));
+      cfg.attrs = attr + 1;
+      cfg.numAttrs = 1;
+      AUT_CUDA_TRY(cudaOccupancyMaxActiveClusters(&at_once, kernel, &cfg));
+      cfg.attrs = attr;
+      cfg.numAttrs = 2;
+      if (at_once < 1) at_once = 1;
+    }
+    if (ws->device < kMaxDevices) resident[ws->device].store(at_once);
+  }
+  const uint64_t workers = std::min<uint64_t>(tiles_m * tiles_n, static_cast<uint64_t>(at_once));
+  cfg.gridDim = dim3(static_cast<unsigned>(workers * (Pair ? 2 : 1)));
+  AUT_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, p));
   return AUT_OK;
 }
 
@@ -452,13 +671,14 @@ aut_status gemm_tiles(aut_workspace *ws, const gemm_params &g, int a_code, int b
   p.wait_cycles = ws->wait_cycles;
   p.stall_tile = ws->stall_tile;
   const uint64_t rows = (g.m + kTileM - 1) / kTileM;
-  if (rows * ((g.n + 255) / 256) >= static_cast<uint64_t>(ws->sm_count))
-    return launch_tiles<256>(ws, p, a_code, b_code, stream);
-  if (rows * ((g.n + 127) / 128) >= static_cast<uint64_t>(ws->sm_count))
-    return launch_tiles<128>(ws, p, a_code, b_code, stream);
-  if (rows * ((g.n + 63) / 64) >= static_cast<uint64_t>(ws->sm_count))
-    return launch_tiles<64>(ws, p, a_code, b_code, stream);
-  return launch_tiles<32>(ws, p, a_code, b_code, stream);
+  const uint64_t sms = static_cast<uint64_t>(ws->sm_count);
+  if (rows >= 2 && rows * ((g.n + 255) / 256) * 5 >= sms * 4)
+    return launch_tiles<256, true>(ws, p, a_code, b_code, stream);
+  if (rows * ((g.n + 127) / 128) >= sms)
+    return launch_tiles<128, false>(ws, p, a_code, b_code, stream);
+  if (rows * ((g.n + 63) / 64) >= sms)
+    return launch_tiles<64, false>(ws, p, a_code, b_code, stream);
+  return launch_tiles<32, false>(ws, p, a_code, b_code, stream);
 }
 
 } // namespace aut::scaled

@@ -326,6 +326,47 @@ def test_gemm_strides_and_alignments(ws, m, layout):
     check_gemm(got, a, sa, b, sb, ref.E4M3, ref.E4M3, BF16)
 
 
+@pytest.mark.parametrize("size", [(300, 10300, 200), (513, 7700, 1000), (1000, 2600, 129),
+                                  (130, 30000, 64), (100, 19000, 130), (20, 9500, 300),
+                                  (17, 40000, 16)])
+@pytest.mark.parametrize("codes", [(ref.E4M3, ref.E4M3), (ref.E5M2, ref.E4M3)])
+@pytest.mark.parametrize("type", [FP32, BF16])
+def test_gemm_wide(ws, size, codes, type):
+    m, n, k = size
+    a, sa = operand(m, k, codes[0], 1, m)
+    b, sb = operand(n, k, codes[1], 128, n)
+    got = run_gemm(ws, a, sa, b, sb, *codes, type)
+    check_gemm(got, a, sa, b, sb, *codes, type)
+
+
+@pytest.mark.parametrize("size", [(150, 300, 2000), (300, 10300, 2000)])
+def test_gemm_wait_that_runs_out(size):
+    """A stage whose copies are withheld: NaN, the sticky status, and a context
+    that works on."""
+    w = _lib.Workspace(0)
+    m, n, k = size
+    a, sa = operand(m, k, ref.E4M3, 1, 1)
+    b, sb = operand(n, k, ref.E4M3, 128, 2)
+    w.inject_stall(3, 2_000_000)
+    dev = [torch.from_numpy(v).cuda() for v in (a, sa, b, sb)]
+    out = torch.zeros(m, n, device="cuda")
+
+    def product():
+        w.gemm_scaled(0, 0, FP32, dev[0].data_ptr(), k, dev[1].data_ptr(), sa.shape[1],
+                      dev[2].data_ptr(), k, dev[3].data_ptr(), sb.shape[1], m, n, k,
+                      out.data_ptr(), n)
+        torch.cuda.synchronize()
+
+    product()
+    assert w.status() == _lib.STATUS_WAIT_TIMEOUT
+    assert torch.isnan(out).any()
+    w.inject_stall()
+    product()
+    assert w.status() == 0
+    check_gemm(out.double().cpu().numpy(), a, sa, b, sb, 0, 0, FP32)
+    w.close()
+
+
 @pytest.mark.parametrize("m", [1, 4, 24, 100, 300])
 def test_gemm_many_blocks_of_k(ws, m):
     a, sa = operand(m, 20000, ref.E4M3, 1, 3)
