@@ -23,10 +23,6 @@ namespace {
 
 constexpr int kMaxDevices = 16;
 constexpr int kTileM = 128;
-constexpr int kEpilogueWarps = 8;
-constexpr int kLoadWarp = kEpilogueWarps, kProductWarp = kEpilogueWarps + 1,
-              kScaleWarp = kEpilogueWarps + 2; // and the next, one for each side
-constexpr int kTileThreads = 32 * (kEpilogueWarps + 4);
 // Blocks of k whose scales are brought at a time, and how many such batches
 // there is room for.
 constexpr int kScaleBatch = 4, kScaleSlots = 4;
@@ -102,6 +98,16 @@ __device__ __forceinline__ void bar_arrive_leader(uint64_t *bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(
                    leader_addr(bar))
                : "memory");
+}
+
+// One lane of a converged warp.
+__device__ __forceinline__ bool elected() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\t"
+               "elect.sync _|p, 0xffffffff;\n\t"
+               "selp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(one));
+  return one != 0;
 }
 
 __device__ __forceinline__ void pair_sync() {
@@ -206,14 +212,6 @@ template <bool Pair, int Columns> __device__ __forceinline__ void tmem_free(uint
   "+f"(v[o]), "+f"(v[o + 1]), "+f"(v[o + 2]), "+f"(v[o + 3]), "+f"(v[o + 4]), "+f"(v[o + 5]), \
       "+f"(v[o + 6]), "+f"(v[o + 7])
 
-__device__ __forceinline__ void tmem_load(float (&v)[32], uint32_t addr) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-               "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-               "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, "
-               "[%32];"
-               : AUT_R8(v, 0), AUT_R8(v, 8), AUT_R8(v, 16), AUT_R8(v, 24)
-               : "r"(addr));
-}
 __device__ __forceinline__ void tmem_load(float (&v)[16], uint32_t addr) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
                "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
@@ -221,10 +219,6 @@ __device__ __forceinline__ void tmem_load(float (&v)[16], uint32_t addr) {
                : "r"(addr));
 }
 // Naming the values keeps their uses behind the wait.
-__device__ __forceinline__ void tmem_wait(float (&v)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : AUT_W8(v, 0), AUT_W8(v, 8), AUT_W8(v, 16), AUT_W8(v, 24)::"memory");
-}
 __device__ __forceinline__ void tmem_wait(float (&v)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" : AUT_W8(v, 0), AUT_W8(v, 8)::"memory");
 }
@@ -268,10 +262,7 @@ __device__ __forceinline__ void store_eight(const tile_params &p, uint64_t i, ui
 
 // BN columns of out by 128 rows for each block; the two blocks of a pair share
 // the columns, and each holds half of the rows of b that they stand for.
-// Tensor memory holds the products of kDepth blocks of k.  With 256 columns
-// that is two, too few to hide the way from the products to the epilogue and
-// back; there each side of the columns is a unit of its own, made, read and
-// given back by itself.
+// Tensor memory holds the products of kDepth blocks of k.
 template <int BN, bool Pair> struct tile_shape {
   static constexpr int kABytes = kTileM * kBlock;
   static constexpr int kBRows = Pair ? BN / 2 : BN;
@@ -279,10 +270,15 @@ template <int BN, bool Pair> struct tile_shape {
   static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr int kStages = 192 * 1024 / kStageBytes < 8 ? 192 * 1024 / kStageBytes : 8;
   static constexpr int kSmem = kStages * kStageBytes + 1024;
+  // Epilogue warps: four to a scheduler for the wide tiles, so that some read
+  // tensor memory while others add (4096 x 8192 x 8192: 865 cycles a block of
+  // k and tile where two to a scheduler took 962; the products alone, 513).
+  static constexpr int kEpilogueWarps = BN >= 128 ? 16 : 8;
+  static constexpr int kParts = kEpilogueWarps / 4; // of the columns
+  static constexpr int kLoadWarp = kEpilogueWarps, kProductWarp = kEpilogueWarps + 1,
+                       kScaleWarp = kEpilogueWarps + 2; // and the next, one for each side
+  static constexpr int kThreads = 32 * (kEpilogueWarps + 4);
   static constexpr int kDepth = BN == 256 ? 2 : 4;
-  static constexpr int kSides = 1; // units of a block of k
-  static constexpr int kUnits = kDepth * kSides;
-  static constexpr int kUnitColumns = BN / kSides;
   static constexpr int kTmemColumns = kDepth * BN;
   static constexpr int kTileRows = Pair ? 2 * kTileM : kTileM; // of out, by both blocks
 };
@@ -302,7 +298,7 @@ __device__ __forceinline__ void tile_at(uint32_t tile, const tile_params &p, uin
 }
 
 template <int BN, bool Pair>
-__global__ void __launch_bounds__(kTileThreads, 1)
+__global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
     tiles_kernel(const __grid_constant__ CUtensorMap map_a,
                  const __grid_constant__ CUtensorMap map_b, const tile_params p) {
   using shape = tile_shape<BN, Pair>;
@@ -311,7 +307,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   unsigned char *ring = reinterpret_cast<unsigned char *>(
       (reinterpret_cast<uintptr_t>(dynamic) + 1023) & ~uintptr_t{1023});
   __shared__ __align__(8) uint64_t full[kStages], empty[kStages];
-  __shared__ __align__(8) uint64_t made[shape::kUnits], taken[shape::kUnits];
+  __shared__ __align__(8) uint64_t made[shape::kDepth], taken[shape::kDepth];
   __shared__ __align__(8) uint64_t scales_in[2][kScaleSlots], scales_used[2][kScaleSlots];
   __shared__ __align__(8) uint64_t drained;
   __shared__ float scales[2][kScaleSlots][kScaleBatch][kTileM]; // of both operands, by sides
@@ -319,7 +315,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   __shared__ int gave_up_word;
   volatile int *gave_up = &gave_up_word;
 
-  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  // the same for all lanes, and known to be
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x / 32), 0);
+  const int lane = threadIdx.x & 31;
   const uint32_t rank = Pair ? blockIdx.x % 2 : 0;
   const uint32_t worker = Pair ? blockIdx.x / 2 : blockIdx.x;
   const uint32_t workers = Pair ? gridDim.x / 2 : gridDim.x;
@@ -328,27 +326,27 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       bar_init(&full[s], 1);
       bar_init(&empty[s], 1);
     }
-    for (int u = 0; u < shape::kUnits; ++u) {
+    for (int u = 0; u < shape::kDepth; ++u) {
       bar_init(&made[u], 1);
-      bar_init(&taken[u], (Pair ? 2 : 1) * kEpilogueWarps / shape::kSides);
+      bar_init(&taken[u], (Pair ? 2 : 1) * shape::kEpilogueWarps);
     }
     for (int side = 0; side < 2; ++side)
       for (int s = 0; s < kScaleSlots; ++s) {
         bar_init(&scales_in[side][s], 1);
-        bar_init(&scales_used[side][s], kEpilogueWarps / 2);
+        bar_init(&scales_used[side][s], shape::kEpilogueWarps / 2);
       }
     bar_init(&drained, 1);
     gave_up_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == kProductWarp) {
+  if (warp == shape::kProductWarp) {
     tmem_alloc<Pair, shape::kTmemColumns>(&tmem_base);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   }
   __syncthreads();
   if (Pair) pair_sync(); // the barriers of both blocks are there
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = tmem_base;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
 
   aut::dev::pdl_wait();
   aut::dev::pdl_release();
@@ -356,18 +354,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const uint32_t tiles = p.tiles_m * p.tiles_n;
   const uint32_t blocks = static_cast<uint32_t>((p.g.k + kBlock - 1) / kBlock);
   uint64_t loads = 0; // by the loading thread
-  if (warp >= kEpilogueWarps) {
-    // 12 warps were launched with 168 registers a thread: 8 x 200 + 4 x 104
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-    if (warp == kLoadWarp && lane == 0) {
+  if (warp >= shape::kEpilogueWarps) {
+    if constexpr (shape::kEpilogueWarps == 8)
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 104;"); // 3 x 168 = 2 x 200 + 104
+    else
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 64;"); // 5 x 96 = 4 x 104 + 64
+    if (warp == shape::kLoadWarp && lane == 0) {
       int s = 0;
       uint32_t parity = 1; // of the wait for a free stage; at first all are
       for (uint32_t tile = worker; tile < tiles && *gave_up == 0; tile += workers) {
         uint32_t tm, tn;
         tile_at<shape::kTileRows>(tile, p, tm, tn);
         const int a_row = static_cast<int>(tm * shape::kTileRows + rank * kTileM);
-        const int b_row =
-            static_cast<int>(tn * BN + rank * (shape::kBRows / shape::kSides));
+        const int b_row = static_cast<int>(tn * BN + rank * shape::kBRows);
         for (uint32_t block = 0; block < blocks; ++block) {
           if (!bar_wait(&empty[s], parity, p.wait_cycles, gave_up)) {
             *gave_up = 1;
@@ -379,50 +378,48 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           if (loads != p.stall_tile) {
             const int column = static_cast<int>(block * kBlock);
             load_tile<Pair>(stage, &map_a, column, a_row, bar);
-#pragma unroll
-            for (int side = 0; side < shape::kSides; ++side)
-              load_tile<Pair>(stage + shape::kABytes + side * (shape::kBBytes / shape::kSides),
-                              &map_b, column, b_row + side * shape::kUnitColumns, bar);
+            load_tile<Pair>(stage + shape::kABytes, &map_b, column, b_row, bar);
           }
           ++loads;
           if (++s == kStages) s = 0, parity ^= 1;
         }
       }
     }
-    if (warp == kProductWarp && lane == 0 && rank == 0) {
+    if (warp == shape::kProductWarp && rank == 0) {
+      // The whole warp goes through the loop and one lane issues: in a branch of
+      // one lane the compiler would move every operand of every product into
+      // the uniform registers that the instruction takes.
       const uint32_t a0 = descriptor_low(smem_addr(ring));
       int s = 0, depth = 0;
       uint32_t parity = 0, free_parity = 1; // tensor memory is all free at first
-      for (uint32_t tile = worker; tile < tiles && *gave_up == 0; tile += workers) {
+      bool ok = true;
+      for (uint32_t tile = worker; tile < tiles && ok; tile += workers) {
         for (uint32_t block = 0; block < blocks; ++block) {
-          const uint32_t a = a0 + s * (shape::kStageBytes >> 4);
-          bool ok = bar_wait(&full[s], parity, p.wait_cycles, gave_up);
-#pragma unroll
-          for (int side = 0; side < shape::kSides; ++side) {
-            const int u = depth * shape::kSides + side;
-            ok = ok && bar_wait(&taken[u], free_parity, p.wait_cycles, gave_up);
-            if (!ok) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            mma_block<Pair>(
-                tmem + u * shape::kUnitColumns, a,
-                a + ((shape::kABytes + side * (shape::kBBytes / shape::kSides)) >> 4), p.idesc);
-            mma_commit<Pair>(&made[u]);
+          // both looked at before either is waited for
+          const bool in = bar_try(smem_addr(&full[s]), parity);
+          const bool room = bar_try(smem_addr(&taken[depth]), free_parity);
+          ok = (in || bar_wait(&full[s], parity, p.wait_cycles, gave_up)) &&
+               (room || bar_wait(&taken[depth], free_parity, p.wait_cycles, gave_up));
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          if (elected()) {
+            const uint32_t a = a0 + s * (shape::kStageBytes >> 4);
+            mma_block<Pair>(tmem + depth * BN, a, a + (shape::kABytes >> 4), p.idesc);
+            mma_commit<Pair>(&made[depth]);
+            mma_commit<Pair>(&empty[s]);
           }
-          if (!ok) {
-            *gave_up = 1;
-            break;
-          }
-          mma_commit<Pair>(&empty[s]);
           if (++s == kStages) s = 0, parity ^= 1;
           if (++depth == shape::kDepth) depth = 0, free_parity ^= 1;
         }
       }
+      if (!ok) *gave_up = 1;
     }
-    if (warp >= kScaleWarp) {
+    if (warp >= shape::kScaleWarp) {
       // a_scale * b_scale of 128 rows and one side of the columns, four rows a
       // lane, a batch of blocks at a time
-      const int side = warp - kScaleWarp;
-      uint64_t batch = 0;
+      const int side = warp - shape::kScaleWarp;
+      uint32_t batch = 0;
       bool ok = true;
       for (uint32_t tile = worker; tile < tiles && ok; tile += workers) {
         uint32_t tm, tn;
@@ -443,12 +440,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             sa += p.g.a_scale_stride;
             sb += p.g.b_scale_stride;
           }
-          const int slot = static_cast<int>(batch % kScaleSlots);
-          ok = batch < kScaleSlots ||
-               bar_wait(&scales_used[side][slot],
-                        static_cast<uint32_t>(batch / kScaleSlots - 1) & 1u, p.wait_cycles, gave_up);
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
+          const uint32_t slot = batch % kScaleSlots;
+          ok = batch < kScaleSlots || lane > 0 ||
+               bar_wait(&scales_used[side][slot], (batch / kScaleSlots - 1) & 1u, p.wait_cycles,
+                        gave_up);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) {
             *gave_up = 1;
             break;
           }
@@ -463,14 +460,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    // Warps w and w + 4 take the tensor-memory lanes (rows of the tile)
-    // 32 (w % 4) ..., each one side of the columns.
-    constexpr int kColumns = BN / 2;
-    constexpr int kChunk = kColumns < 32 ? kColumns : 32;
+    if constexpr (shape::kEpilogueWarps == 8)
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    else
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    // Warps w, w + 4, ... take the tensor-memory lanes (rows of the tile)
+    // 32 (w % 4) ..., each a part of the columns.
+    constexpr int kColumns = BN / shape::kParts;
+    constexpr int kChunk = kColumns < 16 ? kColumns : 16;
     constexpr int kChunks = kColumns / kChunk;
-    const int row = warp % 4 * 32 + lane, side = warp / 4;
-    const uint32_t tmem_own = tmem + (static_cast<uint32_t>(warp % 4 * 32) << 16) + side * kColumns;
+    const int row = warp % 4 * 32 + lane, part = warp / 4, side = part * 2 / shape::kParts;
+    const uint32_t tmem_own = tmem + (static_cast<uint32_t>(warp % 4 * 32) << 16) + part * kColumns;
     uint32_t step = 0, batch = 0;
     bool lost = false;
     for (uint32_t tile = worker; tile < tiles; tile += workers) {
@@ -482,11 +482,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       for (uint32_t block = 0; block < blocks; ++block, ++step) {
         const uint32_t at = block % kScaleBatch, slot = batch % kScaleSlots;
         const uint32_t depth = step % shape::kDepth;
-        const uint32_t u = shape::kSides == 2 ? depth * 2 + side : depth;
         bool ok = at != 0 || bar_wait(&scales_in[side][slot], batch / kScaleSlots & 1u,
                                       p.wait_cycles, gave_up);
         const float s = scales[side][slot][at][row];
-        ok = ok && bar_wait(&made[u], step / shape::kDepth & 1u, p.wait_cycles, gave_up);
+        ok = ok && bar_wait(&made[depth], step / shape::kDepth & 1u, p.wait_cycles, gave_up);
         if (!__all_sync(0xffffffffu, ok)) {
           lost = true;
           break;
@@ -496,20 +495,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           ++batch;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        float v[2][kChunk];
-        tmem_load(v[0], tmem_own + depth * BN);
 #pragma unroll
         for (int c0 = 0; c0 < kChunks; ++c0) {
-          float(&now)[kChunk] = v[c0 % 2];
+          float now[kChunk];
+          tmem_load(now, tmem_own + depth * BN + c0 * kChunk);
           tmem_wait(now);
-          if (c0 + 1 < kChunks) {
-            tmem_load(v[(c0 + 1) % 2], tmem_own + depth * BN + (c0 + 1) * kChunk);
-          } else {
+          if (c0 + 1 == kChunks) {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) {
-              if (Pair) bar_arrive_leader(&taken[u]);
-              else bar_arrive(&taken[u]);
+              if (Pair) bar_arrive_leader(&taken[depth]);
+              else bar_arrive(&taken[depth]);
             }
           }
 #pragma unroll
@@ -525,7 +521,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           acc[c] = make_float2(__int_as_float(0x7fffffff), __int_as_float(0x7fffffff));
       }
       const uint64_t i = uint64_t{tm} * shape::kTileRows + rank * kTileM + row;
-      const uint64_t j0 = uint64_t{tn} * BN + side * kColumns;
+      const uint64_t j0 = uint64_t{tn} * BN + part * kColumns;
       if (i < p.g.m) {
 #pragma unroll
         for (int c = 0; c < kColumns; c += 8) store_eight(p, i, j0 + c, acc + c / 2);
@@ -538,7 +534,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     // loads, which in a pair only the first block's barriers show, and the
     // products.
     int none = 0;
-    if (warp == kLoadWarp && lane == 0) {
+    if (warp == shape::kLoadWarp && lane == 0) {
       atomicOr(p.status, static_cast<unsigned int>(AUT_STATUS_WAIT_TIMEOUT));
       if (Pair) {
         const long long start = clock64();
@@ -551,7 +547,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                      &none);
       }
     }
-    if (warp == kProductWarp && lane == 0 && rank == 0) {
+    if (warp == shape::kProductWarp && lane == 0 && rank == 0) {
       mma_commit<Pair>(&drained);
       bar_wait(&drained, 0, p.wait_cycles, &none);
     }
@@ -559,7 +555,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
   // no block of a pair leaves before the other is done with its barriers
   if (Pair) pair_sync();
-  if (warp == kProductWarp) {
+  if (warp == shape::kProductWarp) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     tmem_free<Pair, shape::kTmemColumns>(tmem);
   }
@@ -610,8 +606,7 @@ aut_status launch_tiles(aut_workspace *ws, tile_params p, int a_code, int b_code
   auto kernel = tiles_kernel<BN, Pair>;
   CUtensorMap map_a, map_b;
   aut_status st = make_map(&map_a, p.g.a, p.g.m, p.g.k, p.g.a_stride, kTileM);
-  if (st == AUT_OK) st = make_map(&map_b, p.g.b, p.g.n, p.g.k, p.g.b_stride,
-                                  shape::kBRows / shape::kSides);
+  if (st == AUT_OK) st = make_map(&map_b, p.g.b, p.g.n, p.g.k, p.g.b_stride, shape::kBRows);
   if (st != AUT_OK) return st;
   const uint64_t tiles_m = (p.g.m + shape::kTileRows - 1) / shape::kTileRows;
   const uint64_t tiles_n = (p.g.n + BN - 1) / BN;
@@ -619,12 +614,12 @@ aut_status launch_tiles(aut_workspace *ws, tile_params p, int a_code, int b_code
     return aut::lib::fail(AUT_ERR_TOO_LARGE, "more than 2^31 - 1 tiles of the product");
   p.tiles_m = static_cast<uint32_t>(tiles_m);
   p.tiles_n = static_cast<uint32_t>(tiles_n);
-  // FP32 sums, both operands with k contiguous, units of kTileRows x kUnitColumns
+  // FP32 sums, both operands with k contiguous, tiles of kTileRows x BN
   p.idesc = (1u << 4) | (static_cast<uint32_t>(a_code) << 7) |
-            (static_cast<uint32_t>(b_code) << 10) | (static_cast<uint32_t>(shape::kUnitColumns / 8) << 17) |
+            (static_cast<uint32_t>(b_code) << 10) | (static_cast<uint32_t>(BN / 8) << 17) |
             (static_cast<uint32_t>(shape::kTileRows / 16) << 24);
   cudaLaunchConfig_t cfg{};
-  cfg.blockDim = dim3(kTileThreads);
+  cfg.blockDim = dim3(shape::kThreads);
   cfg.dynamicSmemBytes = shape::kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2] = {};
