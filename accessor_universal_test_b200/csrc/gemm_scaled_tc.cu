@@ -8,9 +8,9 @@
 // scales, to the sums in the epilogue warps' registers, while the next blocks'
 // products are made elsewhere in tensor memory.
 //
-// Roles: warps 0-7 scale and add and, at the end of a tile, store; of the
-// last warpgroup, one warp loads the operands' tiles, one issues the products
-// and two bring the scales.
+// Roles: the first warps scale and add and, at the end of a tile, store; of the
+// last warpgroup, one warp loads the operands' tiles, one brings the scales and
+// two issue the products.
 #include "gemm_scaled.cuh"
 
 #include <cuda.h>
@@ -275,10 +275,11 @@ template <int BN, bool Pair> struct tile_shape {
   // k and tile where two to a scheduler took 962; the products alone, 513).
   static constexpr int kEpilogueWarps = BN >= 128 ? 16 : 8;
   static constexpr int kParts = kEpilogueWarps / 4; // of the columns
-  static constexpr int kLoadWarp = kEpilogueWarps, kProductWarp = kEpilogueWarps + 1,
-                       kScaleWarp = kEpilogueWarps + 2; // and the next, one for each side
+  static constexpr int kLoadWarp = kEpilogueWarps, kScaleWarp = kEpilogueWarps + 1,
+                       kProductWarp = kEpilogueWarps + 2; // and the next
   static constexpr int kThreads = 32 * (kEpilogueWarps + 4);
   static constexpr int kDepth = BN == 256 ? 2 : 4;
+  static constexpr int kSides = BN == 256 ? 2 : 1; // column blocks of b's scales
   static constexpr int kTmemColumns = kDepth * BN;
   static constexpr int kTileRows = Pair ? 2 * kTileM : kTileM; // of out, by both blocks
 };
@@ -308,9 +309,10 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
       (reinterpret_cast<uintptr_t>(dynamic) + 1023) & ~uintptr_t{1023});
   __shared__ __align__(8) uint64_t full[kStages], empty[kStages];
   __shared__ __align__(8) uint64_t made[shape::kDepth], taken[shape::kDepth];
-  __shared__ __align__(8) uint64_t scales_in[2][kScaleSlots], scales_used[2][kScaleSlots];
+  __shared__ __align__(8) uint64_t scales_in[kScaleSlots], scales_used[kScaleSlots];
   __shared__ __align__(8) uint64_t drained;
-  __shared__ float scales[2][kScaleSlots][kScaleBatch][kTileM]; // of both operands, by sides
+  // of both operands multiplied, for either side of the columns
+  __shared__ float scales[shape::kSides][kScaleSlots][kScaleBatch][kTileM];
   __shared__ uint32_t tmem_base;
   __shared__ int gave_up_word;
   volatile int *gave_up = &gave_up_word;
@@ -330,16 +332,15 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
       bar_init(&made[u], 1);
       bar_init(&taken[u], (Pair ? 2 : 1) * shape::kEpilogueWarps);
     }
-    for (int side = 0; side < 2; ++side)
-      for (int s = 0; s < kScaleSlots; ++s) {
-        bar_init(&scales_in[side][s], 1);
-        bar_init(&scales_used[side][s], shape::kEpilogueWarps / 2);
-      }
-    bar_init(&drained, 1);
+    for (int s = 0; s < kScaleSlots; ++s) {
+      bar_init(&scales_in[s], 1);
+      bar_init(&scales_used[s], shape::kEpilogueWarps);
+    }
+    bar_init(&drained, 2);
     gave_up_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == shape::kProductWarp) {
+  if (warp == shape::kLoadWarp) {
     tmem_alloc<Pair, shape::kTmemColumns>(&tmem_base);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   }
@@ -385,29 +386,34 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
         }
       }
     }
-    if (warp == shape::kProductWarp && rank == 0) {
-      // The whole warp goes through the loop and one lane issues: in a branch of
-      // one lane the compiler would move every operand of every product into
-      // the uniform registers that the instruction takes.
+    if (warp >= shape::kProductWarp && rank == 0) {
+      // Two warps issue the products of every other block: what a warp spends
+      // from block to block (two waits, four products and two arrivals, about
+      // 500 cycles one after the other) is longer than the products of a narrow
+      // tile, and no product adds to another's.  The whole warp goes through
+      // the loop and one lane issues: in a branch of one lane the compiler
+      // would move every operand of every product into the uniform registers
+      // that the instruction takes.
       const uint32_t a0 = descriptor_low(smem_addr(ring));
       int s = 0, depth = 0;
       uint32_t parity = 0, free_parity = 1; // tensor memory is all free at first
+      int turn = warp - shape::kProductWarp; // 0: this warp's
       bool ok = true;
       for (uint32_t tile = worker; tile < tiles && ok; tile += workers) {
-        for (uint32_t block = 0; block < blocks; ++block) {
-          // both looked at before either is waited for
-          const bool in = bar_try(smem_addr(&full[s]), parity);
-          const bool room = bar_try(smem_addr(&taken[depth]), free_parity);
-          ok = (in || bar_wait(&full[s], parity, p.wait_cycles, gave_up)) &&
-               (room || bar_wait(&taken[depth], free_parity, p.wait_cycles, gave_up));
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          if (elected()) {
-            const uint32_t a = a0 + s * (shape::kStageBytes >> 4);
-            mma_block<Pair>(tmem + depth * BN, a, a + (shape::kABytes >> 4), p.idesc);
-            mma_commit<Pair>(&made[depth]);
-            mma_commit<Pair>(&empty[s]);
+        for (uint32_t block = 0; block < blocks; ++block, turn ^= 1) {
+          if (turn == 0) {
+            ok = bar_wait(&full[s], parity, p.wait_cycles, gave_up) &&
+                 bar_wait(&taken[depth], free_parity, p.wait_cycles, gave_up);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (elected()) {
+              const uint32_t a = a0 + s * (shape::kStageBytes >> 4);
+              mma_block<Pair>(tmem + depth * BN, a, a + (shape::kABytes >> 4), p.idesc);
+              mma_commit<Pair>(&made[depth]);
+              mma_commit<Pair>(&empty[s]);
+            }
+            __syncwarp();
           }
           if (++s == kStages) s = 0, parity ^= 1;
           if (++depth == shape::kDepth) depth = 0, free_parity ^= 1;
@@ -415,35 +421,41 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
       }
       if (!ok) *gave_up = 1;
     }
-    if (warp >= shape::kScaleWarp) {
-      // a_scale * b_scale of 128 rows and one side of the columns, four rows a
-      // lane, a batch of blocks at a time
-      const int side = warp - shape::kScaleWarp;
+    if (warp == shape::kScaleWarp) {
+      // a_scale * b_scale of 128 rows and either side of the columns, four rows
+      // a lane, a batch of blocks at a time
       uint32_t batch = 0;
       bool ok = true;
       for (uint32_t tile = worker; tile < tiles && ok; tile += workers) {
         uint32_t tm, tn;
         tile_at<shape::kTileRows>(tile, p, tm, tn);
         const uint64_t i = uint64_t{tm} * shape::kTileRows + rank * kTileM + lane;
-        const uint64_t j = uint64_t{tn} * BN + side * (BN / 2);
+        const uint64_t j = uint64_t{tn} * BN;
         const float *sa = p.g.a_scales + i;
-        const float *sb = p.g.b_scales + (j < p.g.n ? j / kBlock : 0);
+        const float *sb[shape::kSides];
+#pragma unroll
+        for (int side = 0; side < shape::kSides; ++side) {
+          const uint64_t at = j + side * kBlock;
+          sb[side] = p.g.b_scales + (at < p.g.n ? at / kBlock : 0);
+        }
         for (uint32_t block = 0; block < blocks; block += kScaleBatch, ++batch) {
-          float row[kScaleBatch][4], column[kScaleBatch];
+          float row[kScaleBatch][4], column[kScaleBatch][shape::kSides];
 #pragma unroll
           for (int b = 0; b < kScaleBatch; ++b) {
             const bool has = block + b < blocks;
-            column[b] = has ? __ldg(sb) : 0.0f;
+#pragma unroll
+            for (int side = 0; side < shape::kSides; ++side) {
+              column[b][side] = has ? __ldg(sb[side]) : 0.0f;
+              sb[side] += p.g.b_scale_stride;
+            }
 #pragma unroll
             for (int r = 0; r < 4; ++r)
               row[b][r] = has && i + 32 * r < p.g.m ? __ldg(sa + 32 * r) : 0.0f;
             sa += p.g.a_scale_stride;
-            sb += p.g.b_scale_stride;
           }
           const uint32_t slot = batch % kScaleSlots;
-          ok = batch < kScaleSlots || lane > 0 ||
-               bar_wait(&scales_used[side][slot], (batch / kScaleSlots - 1) & 1u, p.wait_cycles,
-                        gave_up);
+          ok = batch < kScaleSlots ||
+               bar_wait(&scales_used[slot], (batch / kScaleSlots - 1) & 1u, p.wait_cycles, gave_up);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) {
             *gave_up = 1;
@@ -452,10 +464,12 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
 #pragma unroll
           for (int b = 0; b < kScaleBatch; ++b)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              scales[side][slot][b][32 * r + lane] = row[b][r] * column[b];
+            for (int side = 0; side < shape::kSides; ++side)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                scales[side][slot][b][32 * r + lane] = row[b][r] * column[b][side];
           __syncwarp();
-          if (lane == 0) bar_arrive(&scales_in[side][slot]);
+          if (lane == 0) bar_arrive(&scales_in[slot]);
         }
       }
     }
@@ -469,7 +483,7 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
     constexpr int kColumns = BN / shape::kParts;
     constexpr int kChunk = kColumns < 16 ? kColumns : 16;
     constexpr int kChunks = kColumns / kChunk;
-    const int row = warp % 4 * 32 + lane, part = warp / 4, side = part * 2 / shape::kParts;
+    const int row = warp % 4 * 32 + lane, part = warp / 4, side = part * shape::kSides / shape::kParts;
     const uint32_t tmem_own = tmem + (static_cast<uint32_t>(warp % 4 * 32) << 16) + part * kColumns;
     uint32_t step = 0, batch = 0;
     bool lost = false;
@@ -482,7 +496,7 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
       for (uint32_t block = 0; block < blocks; ++block, ++step) {
         const uint32_t at = block % kScaleBatch, slot = batch % kScaleSlots;
         const uint32_t depth = step % shape::kDepth;
-        bool ok = at != 0 || bar_wait(&scales_in[side][slot], batch / kScaleSlots & 1u,
+        bool ok = at != 0 || bar_wait(&scales_in[slot], batch / kScaleSlots & 1u,
                                       p.wait_cycles, gave_up);
         const float s = scales[side][slot][at][row];
         ok = ok && bar_wait(&made[depth], step / shape::kDepth & 1u, p.wait_cycles, gave_up);
@@ -491,7 +505,7 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
           break;
         }
         if (at == kScaleBatch - 1 || block + 1 == blocks) {
-          if (lane == 0) bar_arrive(&scales_used[side][slot]);
+          if (lane == 0) bar_arrive(&scales_used[slot]);
           ++batch;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -547,7 +561,7 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
                      &none);
       }
     }
-    if (warp == shape::kProductWarp && lane == 0 && rank == 0) {
+    if (warp >= shape::kProductWarp && lane == 0 && rank == 0) {
       mma_commit<Pair>(&drained);
       bar_wait(&drained, 0, p.wait_cycles, &none);
     }
@@ -555,7 +569,7 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
   }
   // no block of a pair leaves before the other is done with its barriers
   if (Pair) pair_sync();
-  if (warp == shape::kProductWarp) {
+  if (warp == shape::kLoadWarp) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     tmem_free<Pair, shape::kTmemColumns>(tmem);
   }
