@@ -7,9 +7,7 @@ namespace {
 
 // Sixteen codes of a row from column c on; codes at or beyond column k read
 // as zero (what a caller's row padding holds never enters the product).
-template <bool Aligned>
 __device__ __forceinline__ uint4 load_codes(const uint8_t *row, uint64_t c, uint64_t k) {
-  if (Aligned && c + 16 <= k) return __ldg(reinterpret_cast<const uint4 *>(row + c));
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -40,14 +38,28 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
 #undef AUT_MMA
 }
 
-// ---- few rows of a: b streams through registers ---------------------------------
-// A thread block computes 16 rows of b against 8 rows of a; its eight warps
-// share the blocks of k and their sums are joined in warp order.  Both
-// operands go from memory straight into the matrix instruction's registers:
-// the sum over k does not depend on its order, so lane (g, t) takes the 16
-// contiguous codes from 16 t (+ 64) of rows g and g + 8 as its part of two
-// instructions, for both operands alike.
-template <int ACode, int BCode, bool Aligned>
+// Both kernels below take both operands from memory straight into the matrix
+// instruction's registers.  The sum over k does not depend on its order, so lane
+// (g, t) of a warp takes 16 contiguous codes of rows g and g + 8 of b and of row
+// g of a as its part of two instructions, the same ones of both operands.
+
+// Joins the sums of a thread block's eight warps, in warp order, and stores them.
+template <int Rows, int Columns>
+__device__ __forceinline__ void join_warps(const gemm_params &p, const float (&sums)[8][Rows][Columns],
+                                           uint64_t m0, uint64_t n0) {
+  for (int at = threadIdx.x; at < Rows * Columns; at += 256) {
+    const int r = at % Rows, c = at / Rows;
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) s += sums[w][r][c];
+    if (n0 + r < p.n && m0 + c < p.m) store_out(p, m0 + c, n0 + r, s);
+  }
+}
+
+// ---- any alignment -------------------------------------------------------------------
+// A thread block computes 16 rows of b against 8 rows of a; its warps share the
+// blocks of k.  Codes are read byte by byte.
+template <int ACode, int BCode>
 __global__ void __launch_bounds__(256) rows_kernel(const gemm_params p) {
   __shared__ float sums[8][16][8];
   aut::dev::pdl_wait();
@@ -70,9 +82,9 @@ __global__ void __launch_bounds__(256) rows_kernel(const gemm_params p) {
       for (int half = 0; half < 2; ++half) {
         const uint64_t c = block * kBlock + 64 * half + 16 * t;
         const uint4 zero = make_uint4(0, 0, 0, 0);
-        const uint4 u = has_b0 ? load_codes<Aligned>(b0, c, p.k) : zero;
-        const uint4 v = has_b1 ? load_codes<Aligned>(b1, c, p.k) : zero;
-        const uint4 w = has_a ? load_codes<Aligned>(a, c, p.k) : zero;
+        const uint4 u = has_b0 ? load_codes(b0, c, p.k) : zero;
+        const uint4 v = has_b1 ? load_codes(b1, c, p.k) : zero;
+        const uint4 w = has_a ? load_codes(a, c, p.k) : zero;
         mma<BCode, ACode>(d, u.x, v.x, u.y, v.y, w.x, w.y);
         mma<BCode, ACode>(d, u.z, v.z, u.w, v.w, w.z, w.w);
       }
@@ -89,15 +101,129 @@ __global__ void __launch_bounds__(256) rows_kernel(const gemm_params p) {
     sums[warp][g + 8][2 * t] = acc[2];
     sums[warp][g + 8][2 * t + 1] = acc[3];
     __syncthreads();
-    if (threadIdx.x < 128) {
-      const int r = threadIdx.x & 15, c = threadIdx.x >> 4;
-      float s = 0.0f;
-#pragma unroll
-      for (int w = 0; w < 8; ++w) s += sums[w][r][c];
-      if (n0 + r < p.n && m0 + c < p.m) store_out(p, m0 + c, n0 + r, s);
-    }
+    join_warps<16, 8>(p, sums, m0, n0);
     __syncthreads();
   }
+}
+
+// ---- few rows of a -----------------------------------------------------------------
+// The product reads b once and computes little: what counts is how many bytes
+// are under way.  A thread block computes 16 R rows of b against all rows of a
+// (8 T); its eight warps share the blocks of k, four (R = 1) or two at a time,
+// all of whose loads are issued before the first product.
+__device__ __forceinline__ uint4 stream_load(const uint8_t *p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+template <int ACode, int BCode, int R, int T>
+__global__ void __launch_bounds__(256, 2) stream_kernel(const gemm_params p) {
+  constexpr int kAhead = R == 1 && T == 1 ? 4 : 2;
+  __shared__ float sums[8][16 * R][8 * T];
+  aut::dev::pdl_wait();
+  aut::dev::pdl_release();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+  const int g = lane >> 2, t = lane & 3;
+  const uint64_t n0 = uint64_t{blockIdx.x} * (16 * R);
+  const uint32_t blocks = static_cast<uint32_t>((p.k + kBlock - 1) / kBlock);
+  const uint32_t whole = static_cast<uint32_t>(p.k / kBlock);
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  const uint8_t *b[R][2], *a[T];
+  bool has_b[R][2], has_a[T];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint64_t row = n0 + 16 * r + 8 * h + g;
+      has_b[r][h] = row < p.n;
+      b[r][h] = p.b + (has_b[r][h] ? row : 0) * p.b_stride + 16 * t;
+    }
+#pragma unroll
+  for (int i = 0; i < T; ++i) {
+    const uint64_t row = 8 * i + g;
+    has_a[i] = row < p.m;
+    a[i] = p.a + (has_a[i] ? row : 0) * p.a_stride + 16 * t;
+  }
+  float acc[R][T][4] = {};
+  const float *sb = p.b_scales + n0 / kBlock;
+  for (uint32_t first = warp; first < blocks; first += 8 * kAhead) {
+    uint4 u[kAhead][R][2][2], w[kAhead][T][2];
+    float s[kAhead][T][2], column[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const uint32_t block = first + 8 * i;
+      const uint64_t c = uint64_t{block} * kBlock;
+      const bool in = block < whole;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            u[i][r][h][half] = in && has_b[r][h] ? stream_load(b[r][h] + c + 64 * half) : zero;
+#pragma unroll
+        for (int x = 0; x < T; ++x)
+          w[i][x][half] = in && has_a[x]
+                              ? __ldg(reinterpret_cast<const uint4 *>(a[x] + c + 64 * half))
+                              : zero;
+      }
+      column[i] = block < blocks ? __ldg(sb + block * p.b_scale_stride) : 0.0f;
+#pragma unroll
+      for (int x = 0; x < T; ++x)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          s[i][x][e] = block < blocks && 8 * x + 2 * t + e < p.m
+                           ? __ldg(p.a_scales + block * p.a_scale_stride + 8 * x + 2 * t + e)
+                           : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const uint32_t block = first + 8 * i;
+      if (block == whole && whole < blocks) { // the last block, cut short by k
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint64_t c = uint64_t{block} * kBlock + 64 * half + 16 * t;
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (has_b[r][h]) u[i][r][h][half] = load_codes(b[r][h] - 16 * t, c, p.k);
+#pragma unroll
+          for (int x = 0; x < T; ++x)
+            if (has_a[x]) w[i][x][half] = load_codes(a[x] - 16 * t, c, p.k);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int x = 0; x < T; ++x) {
+          float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint4 lo = u[i][r][0][half], hi = u[i][r][1][half], v = w[i][x][half];
+            mma<BCode, ACode>(d, lo.x, hi.x, lo.y, hi.y, v.x, v.y);
+            mma<BCode, ACode>(d, lo.z, hi.z, lo.w, hi.w, v.z, v.w);
+          }
+          const float s0 = s[i][x][0] * column[i], s1 = s[i][x][1] * column[i];
+          acc[r][x][0] = fmaf(d[0], s0, acc[r][x][0]);
+          acc[r][x][1] = fmaf(d[1], s1, acc[r][x][1]);
+          acc[r][x][2] = fmaf(d[2], s0, acc[r][x][2]);
+          acc[r][x][3] = fmaf(d[3], s1, acc[r][x][3]);
+        }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int x = 0; x < T; ++x)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        sums[warp][16 * r + 8 * (e / 2) + g][8 * x + 2 * t + e % 2] = acc[r][x][e];
+  __syncthreads();
+  join_warps<16 * R, 8 * T>(p, sums, 0, n0);
 }
 
 template <class Params>
@@ -118,11 +244,18 @@ aut_status launch(void (*kernel)(Params), uint64_t grid, int max_grid, int threa
 
 template <int ACode, int BCode>
 aut_status gemm_typed(aut_workspace *ws, const gemm_params &p, cudaStream_t stream) {
-  const bool aligned = aligned_operands(p);
-  if (aligned && p.m > 16 && p.k > 0) return gemm_tiles(ws, p, ACode, BCode, stream);
-  const uint64_t tasks = (p.n + 15) / 16 * ((p.m + 7) / 8);
-  return launch(aligned ? rows_kernel<ACode, BCode, true> : rows_kernel<ACode, BCode, false>,
-                tasks, 64 * ws->max_blocks, 256, p, stream);
+  if (!aligned_operands(p) || p.k == 0)
+    return launch(rows_kernel<ACode, BCode>, (p.n + 15) / 16 * ((p.m + 7) / 8),
+                  64 * ws->max_blocks, 256, p, stream);
+  if (p.m > 16) return gemm_tiles(ws, p, ACode, BCode, stream);
+  // 32 rows of b to a block where that still gives every SM one
+  const bool two = (p.n + 31) / 32 >= static_cast<uint64_t>(ws->sm_count);
+  const uint64_t grid = two ? (p.n + 31) / 32 : (p.n + 15) / 16;
+  if (p.m <= 8)
+    return launch(two ? stream_kernel<ACode, BCode, 2, 1> : stream_kernel<ACode, BCode, 1, 1>,
+                  grid, 0x7fffffff, 256, p, stream);
+  return launch(two ? stream_kernel<ACode, BCode, 2, 2> : stream_kernel<ACode, BCode, 1, 2>, grid,
+                0x7fffffff, 256, p, stream);
 }
 
 } // namespace

@@ -17,7 +17,12 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cstdio>
+#include <cstdlib>
 
+#ifndef AUT_KB
+#define AUT_KB 4
+#endif
 namespace aut::scaled {
 namespace {
 
@@ -34,6 +39,10 @@ struct tile_params {
   gemm_params g;
   uint32_t idesc;
   uint32_t tiles_m, tiles_n;
+  uint32_t parts;  // of k, for the split kernels
+  uint32_t a_rows; // of a tile that are loaded: no more than a has, by eights
+  uint32_t stages;      // of the ring, each the operands of a step
+  uint32_t block_bytes; // of one block of k: a_rows of a, then b's rows
   bool wide_out; // out rows take 16-byte stores
   unsigned int *status;
   long long wait_cycles;
@@ -83,11 +92,23 @@ __device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, long lo
   }
 }
 
-// Address, in the pair's shared memory, of what stands at `p` in its first block.
+// Address, in the cluster's shared memory, of what stands at `p` in its first block.
 __device__ __forceinline__ uint32_t leader_addr(const void *p) {
   uint32_t a;
   asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_addr(p)));
   return a;
+}
+
+// Four floats of shared memory of the cluster's block `rank`.
+__device__ __forceinline__ float4 cluster_load(const float *p, uint32_t rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
 }
 
 // Arrives on a barrier of the pair's first block.  Relaxed: what the arrival
@@ -110,7 +131,8 @@ __device__ __forceinline__ bool elected() {
   return one != 0;
 }
 
-__device__ __forceinline__ void pair_sync() {
+// Of all threads of the cluster's blocks.
+__device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\t"
                "barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -262,14 +284,13 @@ __device__ __forceinline__ void store_eight(const tile_params &p, uint64_t i, ui
 
 // BN columns of out by 128 rows for each block; the two blocks of a pair share
 // the columns, and each holds half of the rows of b that they stand for.
-// Tensor memory holds the products of kDepth blocks of k.
+// Tensor memory holds the products of kDepth steps.
 template <int BN, bool Pair> struct tile_shape {
   static constexpr int kABytes = kTileM * kBlock;
   static constexpr int kBRows = Pair ? BN / 2 : BN;
   static constexpr int kBBytes = kBRows * kBlock;
-  static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = 192 * 1024 / kStageBytes < 8 ? 192 * 1024 / kStageBytes : 8;
-  static constexpr int kSmem = kStages * kStageBytes + 1024;
+  static constexpr int kMostStages = 10;
+  static constexpr int kRingBytes = 192 * 1024;
   // Epilogue warps: four to a scheduler for the wide tiles, so that some read
   // tensor memory while others add (4096 x 8192 x 8192: 865 cycles a block of
   // k and tile where two to a scheduler took 962; the products alone, 513).
@@ -278,10 +299,15 @@ template <int BN, bool Pair> struct tile_shape {
   static constexpr int kLoadWarp = kEpilogueWarps, kScaleWarp = kEpilogueWarps + 1,
                        kProductWarp = kEpilogueWarps + 2; // and the next
   static constexpr int kThreads = 32 * (kEpilogueWarps + 4);
-  static constexpr int kDepth = BN == 256 ? 2 : 4;
+  // Blocks of k to a step.  A step costs every role 300 to 500 cycles of waits
+  // and arrivals, more than a narrow tile's products of one block.
+  static constexpr int kBatch = BN <= 64 ? AUT_KB : 1;
+  static constexpr int kDepth = 512 / (kBatch * BN) < 4 ? 512 / (kBatch * BN) : 4;
   static constexpr int kSides = BN == 256 ? 2 : 1; // column blocks of b's scales
-  static constexpr int kTmemColumns = kDepth * BN;
+  static constexpr int kStepColumns = kBatch * BN;
+  static constexpr int kTmemColumns = kDepth * kStepColumns;
   static constexpr int kTileRows = Pair ? 2 * kTileM : kTileM; // of out, by both blocks
+  static constexpr int kJoinPitch = BN + 4; // floats of a row of sums to be joined
 };
 
 // Tiles in bands of rows of tiles (2048 rows of a), column by column within a
@@ -298,16 +324,21 @@ __device__ __forceinline__ void tile_at(uint32_t tile, const tile_params &p, uin
   tn = rest / height;
 }
 
-template <int BN, bool Pair>
+// Split: the blocks of a cluster share a tile's blocks of k, where there are
+// fewer tiles than SMs; each has one tile, and their sums are joined over
+// distributed shared memory in the order of the parts.
+template <int BN, bool Pair, bool Split>
 __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
     tiles_kernel(const __grid_constant__ CUtensorMap map_a,
                  const __grid_constant__ CUtensorMap map_b, const tile_params p) {
   using shape = tile_shape<BN, Pair>;
-  constexpr int kStages = shape::kStages;
+  const int stages = static_cast<int>(p.stages);
+  const uint32_t block_bytes = p.block_bytes, a_bytes = block_bytes - shape::kBBytes;
+  const uint32_t stage_bytes = shape::kBatch * block_bytes;
   extern __shared__ unsigned char dynamic[];
   unsigned char *ring = reinterpret_cast<unsigned char *>(
       (reinterpret_cast<uintptr_t>(dynamic) + 1023) & ~uintptr_t{1023});
-  __shared__ __align__(8) uint64_t full[kStages], empty[kStages];
+  __shared__ __align__(8) uint64_t full[shape::kMostStages], empty[shape::kMostStages];
   __shared__ __align__(8) uint64_t made[shape::kDepth], taken[shape::kDepth];
   __shared__ __align__(8) uint64_t scales_in[kScaleSlots], scales_used[kScaleSlots];
   __shared__ __align__(8) uint64_t drained;
@@ -321,10 +352,11 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x / 32), 0);
   const int lane = threadIdx.x & 31;
   const uint32_t rank = Pair ? blockIdx.x % 2 : 0;
-  const uint32_t worker = Pair ? blockIdx.x / 2 : blockIdx.x;
-  const uint32_t workers = Pair ? gridDim.x / 2 : gridDim.x;
+  const uint32_t shared_by = Pair ? 2 : Split ? p.parts : 1; // blocks to a worker
+  const uint32_t worker = blockIdx.x / shared_by, workers = gridDim.x / shared_by;
+  const uint32_t part = Split ? blockIdx.x % shared_by : 0;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < stages; ++s) {
       bar_init(&full[s], 1);
       bar_init(&empty[s], 1);
     }
@@ -345,62 +377,81 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   }
   __syncthreads();
-  if (Pair) pair_sync(); // the barriers of both blocks are there
+  if (Pair) cluster_sync(); // the barriers of both blocks are there
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
 
+  if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+  }
   aut::dev::pdl_wait();
   aut::dev::pdl_release();
 
   const uint32_t tiles = p.tiles_m * p.tiles_n;
-  const uint32_t blocks = static_cast<uint32_t>((p.g.k + kBlock - 1) / kBlock);
+  // blocks of k: all, or this part's
+  const uint32_t all_blocks = static_cast<uint32_t>((p.g.k + kBlock - 1) / kBlock);
+  const uint32_t each = Split ? (all_blocks + shared_by - 1) / shared_by : all_blocks;
+  const uint32_t first_block = part * each;
+  const uint32_t blocks = !Split ? all_blocks
+                          : first_block >= all_blocks ? 0 : min(each, all_blocks - first_block);
   uint64_t loads = 0; // by the loading thread
   if (warp >= shape::kEpilogueWarps) {
-    if constexpr (shape::kEpilogueWarps == 8)
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 104;"); // 3 x 168 = 2 x 200 + 104
-    else
+    if constexpr (shape::kEpilogueWarps == 16)
       asm volatile("setmaxnreg.dec.sync.aligned.u32 64;"); // 5 x 96 = 4 x 104 + 64
-    if (warp == shape::kLoadWarp && lane == 0) {
+    if (warp == shape::kLoadWarp && lane < 2 * shape::kBatch) {
+      // lane l loads the step's block l / 2, the even lanes of a, the odd of b
+      constexpr uint32_t kLanes = (1u << (2 * shape::kBatch)) - 1;
+      const CUtensorMap *map = lane % 2 == 0 ? &map_a : &map_b;
+      const uint32_t offset = lane / 2 * block_bytes + (lane % 2 == 0 ? 0 : a_bytes);
+      const uint32_t expected =
+          (Pair ? 2 : 1) * shape::kBatch * (p.a_rows * kBlock + shape::kBBytes);
       int s = 0;
       uint32_t parity = 1; // of the wait for a free stage; at first all are
-      for (uint32_t tile = worker; tile < tiles && *gave_up == 0; tile += workers) {
+      bool ok = true;
+      for (uint32_t tile = worker; tile < tiles && ok; tile += workers) {
         uint32_t tm, tn;
         tile_at<shape::kTileRows>(tile, p, tm, tn);
-        const int a_row = static_cast<int>(tm * shape::kTileRows + rank * kTileM);
-        const int b_row = static_cast<int>(tn * BN + rank * shape::kBRows);
-        for (uint32_t block = 0; block < blocks; ++block) {
-          if (!bar_wait(&empty[s], parity, p.wait_cycles, gave_up)) {
+        const int row = static_cast<int>(lane % 2 == 0 ? tm * shape::kTileRows + rank * kTileM
+                                                       : tn * BN + rank * shape::kBRows);
+        for (uint32_t block = 0; block < blocks; block += shape::kBatch) {
+          ok = bar_wait(&empty[s], parity, p.wait_cycles, gave_up);
+          ok = __all_sync(kLanes, ok);
+          if (!ok) {
             *gave_up = 1;
             break;
           }
-          unsigned char *stage = ring + s * shape::kStageBytes;
-          if (rank == 0) bar_expect(&full[s], (Pair ? 2 : 1) * shape::kStageBytes);
+          if (rank == 0 && lane == 0) bar_expect(&full[s], expected);
+          __syncwarp(kLanes);
           const uint32_t bar = Pair ? leader_addr(&full[s]) : smem_addr(&full[s]);
-          if (loads != p.stall_tile) {
-            const int column = static_cast<int>(block * kBlock);
-            load_tile<Pair>(stage, &map_a, column, a_row, bar);
-            load_tile<Pair>(stage + shape::kABytes, &map_b, column, b_row, bar);
-          }
+          if (loads != p.stall_tile)
+            load_tile<Pair>(ring + s * stage_bytes + offset, map,
+                            static_cast<int>((first_block + block + lane / 2) * kBlock), row, bar);
           ++loads;
-          if (++s == kStages) s = 0, parity ^= 1;
+          if (++s == stages) s = 0, parity ^= 1;
         }
       }
     }
     if (warp >= shape::kProductWarp && rank == 0) {
-      // Two warps issue the products of every other block: what a warp spends
-      // from block to block (two waits, four products and two arrivals, about
-      // 500 cycles one after the other) is longer than the products of a narrow
-      // tile, and no product adds to another's.  The whole warp goes through
+      // Two warps issue the products of every other step: what a warp spends
+      // from step to step (two waits, four products a block and two arrivals,
+      // about 500 cycles one after the other) is longer than the products of a narrow
+      // tile, and no product adds to another's.  The stages of the ring and of
+      // tensor memory are even in number, so that each belongs to one of the
+      // warps: a wait tells a barrier's phase from the one before, not from the
+      // one after, and only the warp that waited for a stage's last use knows
+      // that it is over.  The whole warp goes through
       // the loop and one lane issues: in a branch of one lane the compiler
       // would move every operand of every product into the uniform registers
       // that the instruction takes.
+      static_assert(shape::kDepth % 2 == 0 && shape::kMostStages % 2 == 0);
       const uint32_t a0 = descriptor_low(smem_addr(ring));
       int s = 0, depth = 0;
       uint32_t parity = 0, free_parity = 1; // tensor memory is all free at first
       int turn = warp - shape::kProductWarp; // 0: this warp's
       bool ok = true;
       for (uint32_t tile = worker; tile < tiles && ok; tile += workers) {
-        for (uint32_t block = 0; block < blocks; ++block, turn ^= 1) {
+        for (uint32_t block = 0; block < blocks; block += shape::kBatch, turn ^= 1) {
           if (turn == 0) {
             ok = bar_wait(&full[s], parity, p.wait_cycles, gave_up) &&
                  bar_wait(&taken[depth], free_parity, p.wait_cycles, gave_up);
@@ -408,14 +459,19 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (elected()) {
-              const uint32_t a = a0 + s * (shape::kStageBytes >> 4);
-              mma_block<Pair>(tmem + depth * BN, a, a + (shape::kABytes >> 4), p.idesc);
+              uint32_t a = a0 + s * (stage_bytes >> 4), d = tmem + depth * shape::kStepColumns;
+#pragma unroll
+              for (int b = 0; b < shape::kBatch; ++b) {
+                mma_block<Pair>(d, a, a + (a_bytes >> 4), p.idesc);
+                a += block_bytes >> 4;
+                d += BN;
+              }
               mma_commit<Pair>(&made[depth]);
               mma_commit<Pair>(&empty[s]);
             }
             __syncwarp();
           }
-          if (++s == kStages) s = 0, parity ^= 1;
+          if (++s == stages) s = 0, parity ^= 1;
           if (++depth == shape::kDepth) depth = 0, free_parity ^= 1;
         }
       }
@@ -431,12 +487,13 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
         tile_at<shape::kTileRows>(tile, p, tm, tn);
         const uint64_t i = uint64_t{tm} * shape::kTileRows + rank * kTileM + lane;
         const uint64_t j = uint64_t{tn} * BN;
-        const float *sa = p.g.a_scales + i;
+        const float *sa = p.g.a_scales + first_block * p.g.a_scale_stride + i;
         const float *sb[shape::kSides];
 #pragma unroll
         for (int side = 0; side < shape::kSides; ++side) {
           const uint64_t at = j + side * kBlock;
-          sb[side] = p.g.b_scales + (at < p.g.n ? at / kBlock : 0);
+          sb[side] =
+              p.g.b_scales + first_block * p.g.b_scale_stride + (at < p.g.n ? at / kBlock : 0);
         }
         for (uint32_t block = 0; block < blocks; block += kScaleBatch, ++batch) {
           float row[kScaleBatch][4], column[kScaleBatch][shape::kSides];
@@ -474,18 +531,17 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
       }
     }
   } else {
-    if constexpr (shape::kEpilogueWarps == 8)
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    else
+    if constexpr (shape::kEpilogueWarps == 16)
       asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     // Warps w, w + 4, ... take the tensor-memory lanes (rows of the tile)
-    // 32 (w % 4) ..., each a part of the columns.
+    // 32 (w % 4) ..., each a stripe of the columns.
     constexpr int kColumns = BN / shape::kParts;
     constexpr int kChunk = kColumns < 16 ? kColumns : 16;
     constexpr int kChunks = kColumns / kChunk;
-    const int row = warp % 4 * 32 + lane, part = warp / 4, side = part * shape::kSides / shape::kParts;
-    const uint32_t tmem_own = tmem + (static_cast<uint32_t>(warp % 4 * 32) << 16) + part * kColumns;
-    uint32_t step = 0, batch = 0;
+    const int row = warp % 4 * 32 + lane, stripe = warp / 4,
+              side = stripe * shape::kSides / shape::kParts;
+    const uint32_t tmem_own = tmem + (static_cast<uint32_t>(warp % 4 * 32) << 16) + stripe * kColumns;
+    uint32_t depth = 0, made_parity = 0, batch = 0;
     bool lost = false;
     for (uint32_t tile = worker; tile < tiles; tile += workers) {
       uint32_t tm, tn;
@@ -493,27 +549,31 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
       float2 acc[kColumns / 2];
 #pragma unroll
       for (int c = 0; c < kColumns / 2; ++c) acc[c] = make_float2(0.0f, 0.0f);
-      for (uint32_t block = 0; block < blocks; ++block, ++step) {
+      for (uint32_t block = 0; block < blocks; block += shape::kBatch) {
         const uint32_t at = block % kScaleBatch, slot = batch % kScaleSlots;
-        const uint32_t depth = step % shape::kDepth;
-        bool ok = at != 0 || bar_wait(&scales_in[slot], batch / kScaleSlots & 1u,
-                                      p.wait_cycles, gave_up);
-        const float s = scales[side][slot][at][row];
-        ok = ok && bar_wait(&made[depth], step / shape::kDepth & 1u, p.wait_cycles, gave_up);
+        bool ok = at != 0 || bar_wait(&scales_in[slot], batch / kScaleSlots & 1u, p.wait_cycles,
+                                      gave_up);
+        float s[shape::kBatch];
+#pragma unroll
+        for (int b = 0; b < shape::kBatch; ++b) s[b] = scales[side][slot][at + b][row];
+        ok = ok && bar_wait(&made[depth], made_parity, p.wait_cycles, gave_up);
         if (!__all_sync(0xffffffffu, ok)) {
           lost = true;
           break;
         }
-        if (at == kScaleBatch - 1 || block + 1 == blocks) {
+        if (at + shape::kBatch == kScaleBatch || block + shape::kBatch >= blocks) {
           if (lane == 0) bar_arrive(&scales_used[slot]);
           ++batch;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t from = tmem_own + depth * shape::kStepColumns;
 #pragma unroll
         for (int c0 = 0; c0 < kChunks; ++c0) {
-          float now[kChunk];
-          tmem_load(now, tmem_own + depth * BN + c0 * kChunk);
-          tmem_wait(now);
+          float now[shape::kBatch][kChunk];
+#pragma unroll
+          for (int b = 0; b < shape::kBatch; ++b) tmem_load(now[b], from + b * BN + c0 * kChunk);
+#pragma unroll
+          for (int b = 0; b < shape::kBatch; ++b) tmem_wait(now[b]);
           if (c0 + 1 == kChunks) {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
@@ -523,10 +583,13 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
             }
           }
 #pragma unroll
-          for (int c = 0; c < kChunk / 2; ++c)
-            acc[c0 * kChunk / 2 + c] = fma2(make_float2(now[2 * c], now[2 * c + 1]),
-                                            make_float2(s, s), acc[c0 * kChunk / 2 + c]);
+          for (int b = 0; b < shape::kBatch; ++b)
+#pragma unroll
+            for (int c = 0; c < kChunk / 2; ++c)
+              acc[c0 * kChunk / 2 + c] = fma2(make_float2(now[b][2 * c], now[b][2 * c + 1]),
+                                              make_float2(s[b], s[b]), acc[c0 * kChunk / 2 + c]);
         }
+        if (++depth == shape::kDepth) depth = 0, made_parity ^= 1;
       }
       if (lost) {
         *gave_up = 1;
@@ -534,8 +597,17 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
         for (int c = 0; c < kColumns / 2; ++c)
           acc[c] = make_float2(__int_as_float(0x7fffffff), __int_as_float(0x7fffffff));
       }
+      if constexpr (Split) {
+        // all of this block's products are done: the ring is free for its sums
+        float *sums = reinterpret_cast<float *>(ring) + row * shape::kJoinPitch + stripe * kColumns;
+#pragma unroll
+        for (int c = 0; c < kColumns / 2; c += 2)
+          *reinterpret_cast<float4 *>(sums + 2 * c) =
+              make_float4(acc[c].x, acc[c].y, acc[c + 1].x, acc[c + 1].y);
+        break;
+      }
       const uint64_t i = uint64_t{tm} * shape::kTileRows + rank * kTileM + row;
-      const uint64_t j0 = uint64_t{tn} * BN + part * kColumns;
+      const uint64_t j0 = uint64_t{tn} * BN + stripe * kColumns;
       if (i < p.g.m) {
 #pragma unroll
         for (int c = 0; c < kColumns; c += 8) store_eight(p, i, j0 + c, acc + c / 2);
@@ -555,9 +627,9 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
         while (clock64() - start < kPairDrainCycles) {
         }
       } else {
-        for (uint64_t l = loads > kStages ? loads - kStages : 0; l < loads; ++l)
+        for (uint64_t l = loads > p.stages ? loads - p.stages : 0; l < loads; ++l)
           if (l != p.stall_tile)
-            bar_wait(&full[l % kStages], static_cast<uint32_t>(l / kStages) & 1u, p.wait_cycles,
+            bar_wait(&full[l % p.stages], static_cast<uint32_t>(l / p.stages) & 1u, p.wait_cycles,
                      &none);
       }
     }
@@ -567,8 +639,33 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
     }
     __syncthreads();
   }
-  // no block of a pair leaves before the other is done with its barriers
-  if (Pair) pair_sync();
+  if constexpr (Split) {
+    __syncwarp();
+    cluster_sync();
+    // Every block joins a share of the rows: its threads take eight columns of
+    // a row at a time.
+    uint32_t tm, tn;
+    tile_at<shape::kTileRows>(worker, p, tm, tn);
+    const uint64_t i0 = uint64_t{tm} * kTileM;
+    const uint32_t rows = static_cast<uint32_t>(min(uint64_t{kTileM}, p.g.m - i0));
+    const float *sums = reinterpret_cast<const float *>(ring);
+    for (uint32_t at = threadIdx.x * shared_by + part; at < rows * (BN / 8);
+         at += shared_by * shape::kThreads) {
+      const uint32_t row = at / (BN / 8), column = at % (BN / 8) * 8;
+      float2 v[4] = {};
+      for (uint32_t q = 0; q < shared_by; ++q)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float4 u = cluster_load(sums + row * shape::kJoinPitch + column + 4 * h, q);
+          v[2 * h] = add2(v[2 * h], make_float2(u.x, u.y));
+          v[2 * h + 1] = add2(v[2 * h + 1], make_float2(u.z, u.w));
+        }
+      store_eight(p, i0 + row, uint64_t{tn} * BN + column, v);
+    }
+  }
+  // no block of a cluster leaves before the others are done with its barriers
+  // and its sums
+  if (Pair || Split) cluster_sync();
   if (warp == shape::kLoadWarp) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     tmem_free<Pair, shape::kTmemColumns>(tmem);
@@ -613,13 +710,16 @@ aut_status make_map(CUtensorMap *map, const uint8_t *codes, uint64_t rows, uint6
   return AUT_OK;
 }
 
-template <int BN, bool Pair>
+template <int BN, bool Pair, bool Split>
 aut_status launch_tiles(aut_workspace *ws, tile_params p, int a_code, int b_code,
                         cudaStream_t stream) {
   using shape = tile_shape<BN, Pair>;
-  auto kernel = tiles_kernel<BN, Pair>;
+  auto kernel = tiles_kernel<BN, Pair, Split>;
   CUtensorMap map_a, map_b;
-  aut_status st = make_map(&map_a, p.g.a, p.g.m, p.g.k, p.g.a_stride, kTileM);
+  // rows of a tile beyond a's are not even filled with zeros: what the products
+  // make of them is not stored
+  p.a_rows = static_cast<uint32_t>(std::min<uint64_t>(kTileM, (p.g.m + 7) / 8 * 8));
+  aut_status st = make_map(&map_a, p.g.a, p.g.m, p.g.k, p.g.a_stride, static_cast<int>(p.a_rows));
   if (st == AUT_OK) st = make_map(&map_b, p.g.b, p.g.n, p.g.k, p.g.b_stride, shape::kBRows);
   if (st != AUT_OK) return st;
   const uint64_t tiles_m = (p.g.m + shape::kTileRows - 1) / shape::kTileRows;
@@ -632,24 +732,35 @@ aut_status launch_tiles(aut_workspace *ws, tile_params p, int a_code, int b_code
   p.idesc = (1u << 4) | (static_cast<uint32_t>(a_code) << 7) |
             (static_cast<uint32_t>(b_code) << 10) | (static_cast<uint32_t>(BN / 8) << 17) |
             (static_cast<uint32_t>(shape::kTileRows / 16) << 24);
+  // The products read 128 rows of a whatever the ring holds of them: the room
+  // behind the last stage is there for that.
+  p.block_bytes = (p.a_rows * kBlock + 1023) / 1024 * 1024 + shape::kBBytes;
+  const uint32_t stage_bytes = shape::kBatch * p.block_bytes;
+  const uint32_t behind =
+      p.block_bytes < static_cast<uint32_t>(shape::kABytes) ? shape::kABytes - p.block_bytes : 0;
+  // even: see where the products are issued
+  p.stages =
+      std::min<uint32_t>(shape::kMostStages, (shape::kRingBytes - behind) / stage_bytes) / 2 * 2;
+  const uint32_t smem = p.stages * stage_bytes + behind + 1024;
+  const unsigned cluster = Pair ? 2 : Split ? p.parts : 1;
   cudaLaunchConfig_t cfg{};
   cfg.blockDim = dim3(shape::kThreads);
-  cfg.dynamicSmemBytes = shape::kSmem;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.x = cluster;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = Pair ? 2 : 1;
-  // once per device and kernel: shared memory, and how many workers run at a time
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  // once per device and kernel: shared memory, and how many pairs run at a time
   static std::atomic<int> resident[kMaxDevices];
   int at_once = ws->device < kMaxDevices ? resident[ws->device].load() : 0;
   if (at_once == 0) {
     AUT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      shape::kSmem));
+                                      shape::kRingBytes + 1024));
     at_once = ws->sm_count;
     if (Pair) {
       cfg.gridDim = dim3(static_cast<unsigned>(ws->sm_count / 2 * 2));
@@ -662,8 +773,10 @@ aut_status launch_tiles(aut_workspace *ws, tile_params p, int a_code, int b_code
     }
     if (ws->device < kMaxDevices) resident[ws->device].store(at_once);
   }
-  const uint64_t workers = std::min<uint64_t>(tiles_m * tiles_n, static_cast<uint64_t>(at_once));
-  cfg.gridDim = dim3(static_cast<unsigned>(workers * (Pair ? 2 : 1)));
+  // a split tile has workers of its own
+  const uint64_t workers =
+      Split ? tiles_m * tiles_n : std::min<uint64_t>(tiles_m * tiles_n, static_cast<uint64_t>(at_once));
+  cfg.gridDim = dim3(static_cast<unsigned>(workers * cluster));
   AUT_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, p));
   return AUT_OK;
 }
@@ -682,12 +795,21 @@ aut_status gemm_tiles(aut_workspace *ws, const gemm_params &g, int a_code, int b
   const uint64_t rows = (g.m + kTileM - 1) / kTileM;
   const uint64_t sms = static_cast<uint64_t>(ws->sm_count);
   if (rows >= 2 && rows * ((g.n + 255) / 256) * 5 >= sms * 4)
-    return launch_tiles<256, true>(ws, p, a_code, b_code, stream);
+    return launch_tiles<256, true, false>(ws, p, a_code, b_code, stream);
+  const char *e = getenv("AUT_PLAN");
+  if (e) {
+    int bn = 0, sp = 0;
+    sscanf(e, "%d,%d", &bn, &sp);
+    p.parts = sp;
+    if (bn == 128) return sp > 1 ? launch_tiles<128, false, true>(ws, p, a_code, b_code, stream) : launch_tiles<128, false, false>(ws, p, a_code, b_code, stream);
+    if (bn == 64) return sp > 1 ? launch_tiles<64, false, true>(ws, p, a_code, b_code, stream) : launch_tiles<64, false, false>(ws, p, a_code, b_code, stream);
+    if (bn == 32) return sp > 1 ? launch_tiles<32, false, true>(ws, p, a_code, b_code, stream) : launch_tiles<32, false, false>(ws, p, a_code, b_code, stream);
+  }
   if (rows * ((g.n + 127) / 128) >= sms)
-    return launch_tiles<128, false>(ws, p, a_code, b_code, stream);
+    return launch_tiles<128, false, false>(ws, p, a_code, b_code, stream);
   if (rows * ((g.n + 63) / 64) >= sms)
-    return launch_tiles<64, false>(ws, p, a_code, b_code, stream);
-  return launch_tiles<32, false>(ws, p, a_code, b_code, stream);
+    return launch_tiles<64, false, false>(ws, p, a_code, b_code, stream);
+  return launch_tiles<32, false, false>(ws, p, a_code, b_code, stream);
 }
 
 } // namespace aut::scaled
