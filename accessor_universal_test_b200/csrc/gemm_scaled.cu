@@ -40,8 +40,8 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
 
 // Both kernels below take both operands from memory straight into the matrix
 // instruction's registers.  The sum over k does not depend on its order, so lane
-// (g, t) of a warp takes 16 contiguous codes of rows g and g + 8 of b and of row
-// g of a as its part of two instructions, the same ones of both operands.
+// (g, t) of a warp takes contiguous codes of rows g and g + 8 of b and of row g
+// of a as its part of two instructions for every 16, the same of both operands.
 
 // Joins the sums of a thread block's eight warps, in warp order, and stores them.
 template <int Rows, int Columns>
@@ -109,29 +109,56 @@ __global__ void __launch_bounds__(256) rows_kernel(const gemm_params p) {
 // ---- few rows of a -----------------------------------------------------------------
 // The product reads b once and computes little: what counts is how many bytes
 // are under way.  A thread block computes 16 R rows of b against all rows of a
-// (8 T); its eight warps share the blocks of k, four (R = 1) or two at a time,
-// all of whose loads are issued before the first product.
-__device__ __forceinline__ uint4 stream_load(const uint8_t *p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
+// (8 T); its eight warps share the blocks of k, kAhead at a time, all of whose
+// loads are issued before the first product.  Measured (m x n x k, GB/s of
+// codes): 1 x 4096 x 4096 with kAhead 1, 2, 3, 4: 3387, 3640, 2963, 2729;
+// 8 x 8192 x 8192: 3763, 4364, 4063, 4004 (registers: fewer blocks to an SM);
+// keeping the next kAhead blocks' loads under way behind each product: 4181.
+
+// 32 codes of a row, in one load or two.  Measured: one load is faster where b is
+// small (1 x 4096 x 4096: 4.1 against 4.7 us), two where it is large (8 x 8192 x
+// 8192: 15.0 against 16.1 us).
+template <bool Wide>
+__device__ __forceinline__ void stream_load(const uint8_t *p, uint4 &v, uint4 &w) {
+  if constexpr (Wide) {
+    asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v8.b32 "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w), "=r"(w.x), "=r"(w.y), "=r"(w.z),
+                   "=r"(w.w)
+                 : "l"(p));
+  } else {
+    asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                 : "l"(p + 16));
+  }
 }
 
-template <int ACode, int BCode, int R, int T>
+template <int ACode, int BCode, int R, int T, bool Wide>
 __global__ void __launch_bounds__(256, 2) stream_kernel(const gemm_params p) {
-  constexpr int kAhead = R == 1 && T == 1 ? 4 : 2;
+  constexpr int kAhead = T == 1 ? 2 : 1;
   __shared__ float sums[8][16 * R][8 * T];
-  aut::dev::pdl_wait();
-  aut::dev::pdl_release();
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
   const int g = lane >> 2, t = lane & 3;
   const uint64_t n0 = uint64_t{blockIdx.x} * (16 * R);
+  // A hint for the second-level cache, which is coherent, so it may come before
+  // the kernels before this one have ended (1 x 4096 x 4096: 6.1 -> 4.6 us with
+  // launches one behind the other): each lane's line of its row pairs' blocks
+  // warp, warp + 8, + 16 and + 24.
+  const uint64_t ahead = (uint64_t{static_cast<uint32_t>(warp)} + 8 * t) * kBlock;
+  if (ahead < p.k)
+#pragma unroll
+    for (int r = 0; r < 2 * R; ++r)
+      if (n0 + 8 * r + g < p.n)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.b + (n0 + 8 * r + g) * p.b_stride + ahead));
+  aut::dev::pdl_wait();
+  aut::dev::pdl_release();
   const uint32_t blocks = static_cast<uint32_t>((p.k + kBlock - 1) / kBlock);
   const uint32_t whole = static_cast<uint32_t>(p.k / kBlock);
   const uint4 zero = make_uint4(0, 0, 0, 0);
-  const uint8_t *b[R][2], *a[T];
+  const uint8_t *b[R][2], *a[T]; // lane (g, t): the codes from 32 t of a block
   bool has_b[R][2], has_a[T];
 #pragma unroll
   for (int r = 0; r < R; ++r)
@@ -139,16 +166,15 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(const gemm_params p) {
     for (int h = 0; h < 2; ++h) {
       const uint64_t row = n0 + 16 * r + 8 * h + g;
       has_b[r][h] = row < p.n;
-      b[r][h] = p.b + (has_b[r][h] ? row : 0) * p.b_stride + 16 * t;
+      b[r][h] = p.b + (has_b[r][h] ? row : 0) * p.b_stride + 32 * t;
     }
 #pragma unroll
   for (int i = 0; i < T; ++i) {
     const uint64_t row = 8 * i + g;
     has_a[i] = row < p.m;
-    a[i] = p.a + (has_a[i] ? row : 0) * p.a_stride + 16 * t;
+    a[i] = p.a + (has_a[i] ? row : 0) * p.a_stride + 32 * t;
   }
   float acc[R][T][4] = {};
-  const float *sb = p.b_scales + n0 / kBlock;
   for (uint32_t first = warp; first < blocks; first += 8 * kAhead) {
     uint4 u[kAhead][R][2][2], w[kAhead][T][2];
     float s[kAhead][T][2], column[kAhead];
@@ -163,14 +189,18 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(const gemm_params p) {
         for (int r = 0; r < R; ++r)
 #pragma unroll
           for (int h = 0; h < 2; ++h)
-            u[i][r][h][half] = in && has_b[r][h] ? stream_load(b[r][h] + c + 64 * half) : zero;
+            if (half == 0) { // both halves at once
+              u[i][r][h][0] = u[i][r][h][1] = zero;
+              if (in && has_b[r][h]) stream_load<Wide>(b[r][h] + c, u[i][r][h][0], u[i][r][h][1]);
+            }
 #pragma unroll
         for (int x = 0; x < T; ++x)
           w[i][x][half] = in && has_a[x]
-                              ? __ldg(reinterpret_cast<const uint4 *>(a[x] + c + 64 * half))
+                              ? __ldg(reinterpret_cast<const uint4 *>(a[x] + c + 16 * half))
                               : zero;
       }
-      column[i] = block < blocks ? __ldg(sb + block * p.b_scale_stride) : 0.0f;
+      column[i] =
+          block < blocks ? __ldg(p.b_scales + n0 / kBlock + block * p.b_scale_stride) : 0.0f;
 #pragma unroll
       for (int x = 0; x < T; ++x)
 #pragma unroll
@@ -185,15 +215,15 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(const gemm_params p) {
       if (block == whole && whole < blocks) { // the last block, cut short by k
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const uint64_t c = uint64_t{block} * kBlock + 64 * half + 16 * t;
+          const uint64_t c = uint64_t{block} * kBlock + 32 * t + 16 * half;
 #pragma unroll
           for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-              if (has_b[r][h]) u[i][r][h][half] = load_codes(b[r][h] - 16 * t, c, p.k);
+              if (has_b[r][h]) u[i][r][h][half] = load_codes(b[r][h] - 32 * t, c, p.k);
 #pragma unroll
           for (int x = 0; x < T; ++x)
-            if (has_a[x]) w[i][x][half] = load_codes(a[x] - 16 * t, c, p.k);
+            if (has_a[x]) w[i][x][half] = load_codes(a[x] - 32 * t, c, p.k);
         }
       }
 #pragma unroll
@@ -242,20 +272,33 @@ aut_status launch(void (*kernel)(Params), uint64_t grid, int max_grid, int threa
   return AUT_OK;
 }
 
+template <int ACode, int BCode, bool Wide>
+aut_status gemm_few(aut_workspace *ws, const gemm_params &p, cudaStream_t stream) {
+  if (p.m <= 8)
+    return launch(stream_kernel<ACode, BCode, 1, 1, Wide>, (p.n + 15) / 16, 0x7fffffff, 256, p,
+                  stream);
+  // 32 rows of b to a block where that still gives every SM one
+  if ((p.n + 31) / 32 >= static_cast<uint64_t>(ws->sm_count))
+    return launch(stream_kernel<ACode, BCode, 2, 2, Wide>, (p.n + 31) / 32, 0x7fffffff, 256, p,
+                  stream);
+  return launch(stream_kernel<ACode, BCode, 1, 2, Wide>, (p.n + 15) / 16, 0x7fffffff, 256, p,
+                stream);
+}
+
 template <int ACode, int BCode>
 aut_status gemm_typed(aut_workspace *ws, const gemm_params &p, cudaStream_t stream) {
-  if (!aligned_operands(p) || p.k == 0)
+  if (!aligned_operands(p, 16) || p.k == 0)
     return launch(rows_kernel<ACode, BCode>, (p.n + 15) / 16 * ((p.m + 7) / 8),
                   64 * ws->max_blocks, 256, p, stream);
   if (p.m > 16) return gemm_tiles(ws, p, ACode, BCode, stream);
-  // 32 rows of b to a block where that still gives every SM one
-  const bool two = (p.n + 31) / 32 >= static_cast<uint64_t>(ws->sm_count);
-  const uint64_t grid = two ? (p.n + 31) / 32 : (p.n + 15) / 16;
-  if (p.m <= 8)
-    return launch(two ? stream_kernel<ACode, BCode, 2, 1> : stream_kernel<ACode, BCode, 1, 1>,
-                  grid, 0x7fffffff, 256, p, stream);
-  return launch(two ? stream_kernel<ACode, BCode, 2, 2> : stream_kernel<ACode, BCode, 1, 2>, grid,
-                0x7fffffff, 256, p, stream);
+  // Measured: up to 8 rows streaming is faster than tiles (8 x 8192 x 8192: 15.0
+  // against 16.4 us, 1 x 4096 x 4096: 4.1 against 6.8); up to 16 it is
+  // where b is small (16 x 4096 x 4096: 6.1 against 7.1 us; 8192 x 8192: 19.5
+  // against 16.4).
+  if (p.m > 8 && p.n * p.k >= uint64_t{1} << 25) return gemm_tiles(ws, p, ACode, BCode, stream);
+  return aligned_operands(p, 32) && p.n * p.k < uint64_t{1} << 25
+             ? gemm_few<ACode, BCode, true>(ws, p, stream)
+             : gemm_few<ACode, BCode, false>(ws, p, stream);
 }
 
 } // namespace

@@ -26,10 +26,10 @@ __device__ __forceinline__ void store_out(const gemm_params &p, uint64_t i, uint
   else static_cast<__half *>(p.out)[at] = narrow<__half>(v);
 }
 
-// Whether both operands start on 16-byte boundaries, row by row.
-inline bool aligned_operands(const gemm_params &p) {
-  return reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && (p.m == 1 || p.a_stride % 16 == 0) &&
-         reinterpret_cast<uintptr_t>(p.b) % 16 == 0 && (p.n == 1 || p.b_stride % 16 == 0);
+// Whether every row of both operands starts on a boundary of `bytes`.
+inline bool aligned_operands(const gemm_params &p, uint64_t bytes) {
+  return reinterpret_cast<uintptr_t>(p.a) % bytes == 0 && (p.m == 1 || p.a_stride % bytes == 0) &&
+         reinterpret_cast<uintptr_t>(p.b) % bytes == 0 && (p.n == 1 || p.b_stride % bytes == 0);
 }
 
 // The tensor-core path over tensor memory (gemm_scaled_tc.cu).

@@ -17,12 +17,7 @@
 
 #include <algorithm>
 #include <atomic>
-#include <cstdio>
-#include <cstdlib>
 
-#ifndef AUT_KB
-#define AUT_KB 4
-#endif
 namespace aut::scaled {
 namespace {
 
@@ -282,6 +277,30 @@ __device__ __forceinline__ void store_eight(const tile_params &p, uint64_t i, ui
   }
 }
 
+// Four neighbouring results.
+__device__ __forceinline__ void store_four(const tile_params &p, uint64_t i, uint64_t j,
+                                           const float2 *v) {
+  const gemm_params &g = p.g;
+  if (p.wide_out && j + 4 <= g.n) {
+    const uint64_t at = i * g.out_stride + j;
+    if (g.type == AUT_TYPE_FP32)
+      *reinterpret_cast<float4 *>(static_cast<float *>(g.out) + at) =
+          make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+    else if (g.type == AUT_TYPE_BF16)
+      *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(g.out) + at) =
+          make_uint2(pack_bf16(v[0].x, v[0].y), pack_bf16(v[1].x, v[1].y));
+    else
+      *reinterpret_cast<uint2 *>(static_cast<__half *>(g.out) + at) =
+          make_uint2(pack_fp16(v[0].x, v[0].y), pack_fp16(v[1].x, v[1].y));
+    return;
+  }
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    if (j + 2 * c < g.n) store_out(g, i, j + 2 * c, v[c].x);
+    if (j + 2 * c + 1 < g.n) store_out(g, i, j + 2 * c + 1, v[c].y);
+  }
+}
+
 // BN columns of out by 128 rows for each block; the two blocks of a pair share
 // the columns, and each holds half of the rows of b that they stand for.
 // Tensor memory holds the products of kDepth steps.
@@ -290,7 +309,7 @@ template <int BN, bool Pair> struct tile_shape {
   static constexpr int kBRows = Pair ? BN / 2 : BN;
   static constexpr int kBBytes = kBRows * kBlock;
   static constexpr int kMostStages = 10;
-  static constexpr int kRingBytes = 192 * 1024;
+  static constexpr int kRingBytes = 208 * 1024;
   // Epilogue warps: four to a scheduler for the wide tiles, so that some read
   // tensor memory while others add (4096 x 8192 x 8192: 865 cycles a block of
   // k and tile where two to a scheduler took 962; the products alone, 513).
@@ -301,13 +320,12 @@ template <int BN, bool Pair> struct tile_shape {
   static constexpr int kThreads = 32 * (kEpilogueWarps + 4);
   // Blocks of k to a step.  A step costs every role 300 to 500 cycles of waits
   // and arrivals, more than a narrow tile's products of one block.
-  static constexpr int kBatch = BN <= 64 ? AUT_KB : 1;
+  static constexpr int kBatch = BN == 32 ? 4 : BN == 64 ? 2 : 1;
   static constexpr int kDepth = 512 / (kBatch * BN) < 4 ? 512 / (kBatch * BN) : 4;
   static constexpr int kSides = BN == 256 ? 2 : 1; // column blocks of b's scales
   static constexpr int kStepColumns = kBatch * BN;
   static constexpr int kTmemColumns = kDepth * kStepColumns;
   static constexpr int kTileRows = Pair ? 2 * kTileM : kTileM; // of out, by both blocks
-  static constexpr int kJoinPitch = BN + 4; // floats of a row of sums to be joined
 };
 
 // Tiles in bands of rows of tiles (2048 rows of a), column by column within a
@@ -332,6 +350,7 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
     tiles_kernel(const __grid_constant__ CUtensorMap map_a,
                  const __grid_constant__ CUtensorMap map_b, const tile_params p) {
   using shape = tile_shape<BN, Pair>;
+  [[maybe_unused]] constexpr int kJoinPitch = BN + 4; // floats of a row of sums to be joined
   const int stages = static_cast<int>(p.stages);
   const uint32_t block_bytes = p.block_bytes, a_bytes = block_bytes - shape::kBBytes;
   const uint32_t stage_bytes = shape::kBatch * block_bytes;
@@ -396,14 +415,18 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
   const uint32_t blocks = !Split ? all_blocks
                           : first_block >= all_blocks ? 0 : min(each, all_blocks - first_block);
   uint64_t loads = 0; // by the loading thread
+  const uint64_t withheld = p.stall_tile / shape::kBatch; // of the loads, by the test hook
   if (warp >= shape::kEpilogueWarps) {
     if constexpr (shape::kEpilogueWarps == 16)
       asm volatile("setmaxnreg.dec.sync.aligned.u32 64;"); // 5 x 96 = 4 x 104 + 64
-    if (warp == shape::kLoadWarp && lane < 2 * shape::kBatch) {
-      // lane l loads the step's block l / 2, the even lanes of a, the odd of b
-      constexpr uint32_t kLanes = (1u << (2 * shape::kBatch)) - 1;
-      const CUtensorMap *map = lane % 2 == 0 ? &map_a : &map_b;
-      const uint32_t offset = lane / 2 * block_bytes + (lane % 2 == 0 ? 0 : a_bytes);
+    constexpr int kLoaders = shape::kBatch == 1 ? 1 : 2 * shape::kBatch;
+    if (warp == shape::kLoadWarp && lane < kLoaders) {
+      // One lane loads both operands of a step of one block; of several blocks,
+      // lane l loads block l / 2, the even lanes of a, the odd of b.
+      constexpr uint32_t kLanes = (1u << kLoaders) - 1;
+      const bool of_a = lane % 2 == 0;
+      const CUtensorMap *map = of_a ? &map_a : &map_b;
+      const uint32_t offset = lane / 2 * block_bytes + (of_a ? 0 : a_bytes);
       const uint32_t expected =
           (Pair ? 2 : 1) * shape::kBatch * (p.a_rows * kBlock + shape::kBBytes);
       int s = 0;
@@ -412,21 +435,29 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
       for (uint32_t tile = worker; tile < tiles && ok; tile += workers) {
         uint32_t tm, tn;
         tile_at<shape::kTileRows>(tile, p, tm, tn);
-        const int row = static_cast<int>(lane % 2 == 0 ? tm * shape::kTileRows + rank * kTileM
-                                                       : tn * BN + rank * shape::kBRows);
+        const int a_row = static_cast<int>(tm * shape::kTileRows + rank * kTileM);
+        const int b_row = static_cast<int>(tn * BN + rank * shape::kBRows);
         for (uint32_t block = 0; block < blocks; block += shape::kBatch) {
           ok = bar_wait(&empty[s], parity, p.wait_cycles, gave_up);
-          ok = __all_sync(kLanes, ok);
+          if constexpr (kLoaders > 1) ok = __all_sync(kLanes, ok);
           if (!ok) {
             *gave_up = 1;
             break;
           }
           if (rank == 0 && lane == 0) bar_expect(&full[s], expected);
-          __syncwarp(kLanes);
+          if constexpr (kLoaders > 1) __syncwarp(kLanes);
           const uint32_t bar = Pair ? leader_addr(&full[s]) : smem_addr(&full[s]);
-          if (loads != p.stall_tile)
-            load_tile<Pair>(ring + s * stage_bytes + offset, map,
-                            static_cast<int>((first_block + block + lane / 2) * kBlock), row, bar);
+          unsigned char *stage = ring + s * stage_bytes;
+          const int column = static_cast<int>((first_block + block) * kBlock);
+          if (loads != withheld) {
+            if constexpr (kLoaders > 1) {
+              load_tile<Pair>(stage + offset, map, column + lane / 2 * kBlock,
+                              of_a ? a_row : b_row, bar);
+            } else {
+              load_tile<Pair>(stage, &map_a, column, a_row, bar);
+              load_tile<Pair>(stage + a_bytes, &map_b, column, b_row, bar);
+            }
+          }
           ++loads;
           if (++s == stages) s = 0, parity ^= 1;
         }
@@ -599,7 +630,7 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
       }
       if constexpr (Split) {
         // all of this block's products are done: the ring is free for its sums
-        float *sums = reinterpret_cast<float *>(ring) + row * shape::kJoinPitch + stripe * kColumns;
+        float *sums = reinterpret_cast<float *>(ring) + row * kJoinPitch + stripe * kColumns;
 #pragma unroll
         for (int c = 0; c < kColumns / 2; c += 2)
           *reinterpret_cast<float4 *>(sums + 2 * c) =
@@ -628,7 +659,7 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
         }
       } else {
         for (uint64_t l = loads > p.stages ? loads - p.stages : 0; l < loads; ++l)
-          if (l != p.stall_tile)
+          if (l != withheld)
             bar_wait(&full[l % p.stages], static_cast<uint32_t>(l / p.stages) & 1u, p.wait_cycles,
                      &none);
       }
@@ -642,25 +673,29 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
   if constexpr (Split) {
     __syncwarp();
     cluster_sync();
-    // Every block joins a share of the rows: its threads take eight columns of
-    // a row at a time.
+    // Every block joins a share of the sums, a thread four columns of a row at a
+    // time, so that a warp reads whole lines of the others' shared memory.
     uint32_t tm, tn;
     tile_at<shape::kTileRows>(worker, p, tm, tn);
-    const uint64_t i0 = uint64_t{tm} * kTileM;
-    const uint32_t rows = static_cast<uint32_t>(min(uint64_t{kTileM}, p.g.m - i0));
+    const uint64_t i0 = uint64_t{tm} * kTileM, j0 = uint64_t{tn} * BN;
+    const uint32_t fours = static_cast<uint32_t>(min(uint64_t{kTileM}, p.g.m - i0)) * (BN / 4);
+    const uint32_t share = (fours + shared_by - 1) / shared_by;
     const float *sums = reinterpret_cast<const float *>(ring);
-    for (uint32_t at = threadIdx.x * shared_by + part; at < rows * (BN / 8);
-         at += shared_by * shape::kThreads) {
-      const uint32_t row = at / (BN / 8), column = at % (BN / 8) * 8;
-      float2 v[4] = {};
-      for (uint32_t q = 0; q < shared_by; ++q)
+    for (uint32_t at = part * share + threadIdx.x; at < min(fours, (part + 1) * share);
+         at += shape::kThreads) {
+      const uint32_t row = at / (BN / 4), column = at % (BN / 4) * 4;
+      float2 v[2] = {};
+      float4 u[8];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float4 u = cluster_load(sums + row * shape::kJoinPitch + column + 4 * h, q);
-          v[2 * h] = add2(v[2 * h], make_float2(u.x, u.y));
-          v[2 * h + 1] = add2(v[2 * h + 1], make_float2(u.z, u.w));
+      for (uint32_t q = 0; q < 8; ++q)
+        if (q < shared_by) u[q] = cluster_load(sums + row * kJoinPitch + column, q);
+#pragma unroll
+      for (uint32_t q = 0; q < 8; ++q)
+        if (q < shared_by) {
+          v[0] = add2(v[0], make_float2(u[q].x, u[q].y));
+          v[1] = add2(v[1], make_float2(u[q].z, u[q].w));
         }
-      store_eight(p, i0 + row, uint64_t{tn} * BN + column, v);
+      store_four(p, i0 + row, j0 + column, v);
     }
   }
   // no block of a cluster leaves before the others are done with its barriers
@@ -792,24 +827,47 @@ aut_status gemm_tiles(aut_workspace *ws, const gemm_params &g, int a_code, int b
   p.status = ws->tickets + aut::lib::kMaxBatchPerLaunch;
   p.wait_cycles = ws->wait_cycles;
   p.stall_tile = ws->stall_tile;
+  // The way is the one that takes the shortest time by what was measured: beside
+  // a start of about 3 us, for every block of k that an SM goes through 0.14 to
+  // 0.18 us with 32 columns (32 and 128 x 4096 x 4096: 7.1 and 8.9 us), 0.2 with
+  // 64 (16 x 8192 x 8192: 16.4), 0.3 with 128 (256 x 8192 x 8192: 24.6), 0.54
+  // for a pair on 256 x 256 (4096 x 8192 x 8192: 258), and to join S parts of k
+  // 0.5 + 0.4 S us (64 x 1024 x 8192 with 64 columns, S = 1, 2, 4: 14.9, 10.3,
+  // 7.5 us).
+  const uint64_t blocks = (g.k + kBlock - 1) / kBlock;
   const uint64_t rows = (g.m + kTileM - 1) / kTileM;
   const uint64_t sms = static_cast<uint64_t>(ws->sm_count);
-  if (rows >= 2 && rows * ((g.n + 255) / 256) * 5 >= sms * 4)
-    return launch_tiles<256, true, false>(ws, p, a_code, b_code, stream);
-  const char *e = getenv("AUT_PLAN");
-  if (e) {
-    int bn = 0, sp = 0;
-    sscanf(e, "%d,%d", &bn, &sp);
-    p.parts = sp;
-    if (bn == 128) return sp > 1 ? launch_tiles<128, false, true>(ws, p, a_code, b_code, stream) : launch_tiles<128, false, false>(ws, p, a_code, b_code, stream);
-    if (bn == 64) return sp > 1 ? launch_tiles<64, false, true>(ws, p, a_code, b_code, stream) : launch_tiles<64, false, false>(ws, p, a_code, b_code, stream);
-    if (bn == 32) return sp > 1 ? launch_tiles<32, false, true>(ws, p, a_code, b_code, stream) : launch_tiles<32, false, false>(ws, p, a_code, b_code, stream);
+  const auto rounds = [](uint64_t work, uint64_t at_once) { return (work + at_once - 1) / at_once; };
+  int columns = 256;
+  double best = 0.54 * blocks * rounds((rows + 1) / 2 * ((g.n + 255) / 256), sms / 2);
+  if (rows == 1) best *= 2; // half of the pair has nothing to do
+  p.parts = 1;
+  const struct {
+    int columns;
+    double block;
+  } kinds[] = {{32, 0.12 + 0.0005 * std::min<uint64_t>(g.m, kTileM)}, {64, 0.2}, {128, 0.3}};
+  for (const auto &kind : kinds) {
+    const uint64_t tiles = rows * ((g.n + kind.columns - 1) / kind.columns);
+    for (uint32_t parts = 1; parts <= 8; parts *= 2) {
+      if (parts > 1 && (tiles * parts > sms || blocks < 2 * parts)) break;
+      const double t = kind.block * rounds(blocks, parts) * rounds(tiles * parts, sms) +
+                       (parts > 1 ? 0.5 + 0.4 * parts : 0);
+      if (t < best) best = t, columns = kind.columns, p.parts = parts;
+    }
   }
-  if (rows * ((g.n + 127) / 128) >= sms)
-    return launch_tiles<128, false, false>(ws, p, a_code, b_code, stream);
-  if (rows * ((g.n + 63) / 64) >= sms)
-    return launch_tiles<64, false, false>(ws, p, a_code, b_code, stream);
-  return launch_tiles<32, false, false>(ws, p, a_code, b_code, stream);
+  const bool split = p.parts > 1;
+  switch (columns) {
+  case 32:
+    return split ? launch_tiles<32, false, true>(ws, p, a_code, b_code, stream)
+                 : launch_tiles<32, false, false>(ws, p, a_code, b_code, stream);
+  case 64:
+    return split ? launch_tiles<64, false, true>(ws, p, a_code, b_code, stream)
+                 : launch_tiles<64, false, false>(ws, p, a_code, b_code, stream);
+  case 128:
+    return split ? launch_tiles<128, false, true>(ws, p, a_code, b_code, stream)
+                 : launch_tiles<128, false, false>(ws, p, a_code, b_code, stream);
+  default: return launch_tiles<256, true, false>(ws, p, a_code, b_code, stream);
+  }
 }
 
 } // namespace aut::scaled
