@@ -192,6 +192,9 @@ aut_status aut_workspace_status(aut_workspace *ws, uint32_t *status,
  * stage therefore runs out: the block lets its other copies land, sets
  * AUT_STATUS_WAIT_TIMEOUT and the DOT's result is NaN.  No copy is left in
  * flight, nothing waits without a bound, and the context stays usable.
+ * aut_gemm_scaled over tiles (more than 16 rows of a) does the same with the
+ * load of the stall_tile-th block of 128 codes that a thread block makes; what
+ * that thread block had still to write is NaN.
  * stall_tile = UINT64_MAX switches the hook off.  Not for production use. */
 aut_status aut_workspace_inject_stall(aut_workspace *ws, uint64_t stall_tile,
                                       uint64_t wait_cycles);

@@ -547,3 +547,53 @@ def test_refusals(ws):
         args[at] = value
         refused(status, text, gemm, *args)
     assert (buf == 0).all() and ws.status() == 0
+
+
+@pytest.mark.parametrize("tokens", [1, 12, 150])
+def test_feed_forward_example(ws, tokens):
+    """The example's block against itself in 64 bits from the decoded weights:
+    what is left is the encoding of the activations and of the output."""
+    import os
+    import sys
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                                    "examples"))
+    import scaled_feed_forward as example
+    g = torch.Generator(device="cuda").manual_seed(tokens)
+    width, inner = 512, 768
+
+    def normal(*shape, scale=1.0):
+        return (torch.randn(*shape, generator=g, device="cuda") * scale).bfloat16()
+
+    gain, x, stream = 1 + normal(width, scale=0.1), normal(tokens, width), normal(tokens, width)
+    up, down = normal(2 * inner, width, scale=width ** -0.5), normal(width, inner, scale=inner ** -0.5)
+    block = example.FeedForward(ws, gain, up, down)
+    before = stream.clone()
+    got = block(x, stream)
+    torch.testing.assert_close(stream, (x.float() + before.float()).bfloat16(), rtol=0, atol=0)
+    want, _ = example.reference(gain, block.up.decoded(), block.down.decoded(), x, before)
+    # codes round within 2^-4 of a value, two encodings one behind the other,
+    # each error spread over the sums: far below half of 2^-4 in the norm
+    assert (got.float() - want).norm() <= 2 ** -4 * want.norm()
+
+
+def test_tensor_calls(ws):
+    from accessor_universal_test_b200 import scaled
+    x = torch.randn(70, 300, device="cuda")
+    a = scaled.encode(ws, x)
+    b = scaled.encode(ws, torch.randn(200, 300, device="cuda"), block_rows=128)
+    assert (a.decoded() - x).abs().max() <= x.abs().max() * 2 ** -4
+    out = scaled.matmul(ws, a, b, dtype=torch.float32)
+    torch.testing.assert_close(out, a.decoded() @ b.decoded().t(), rtol=1e-4, atol=1e-3)
+    same = torch.empty_like(out)
+    assert scaled.matmul(ws, a, b, out=same) is same and torch.equal(same, out)
+    again = scaled.encode(ws, x, out=a)
+    assert again is a
+    n, s = scaled.rms_norm(ws, x)
+    assert s is x and n.codes.shape == (70, 300)
+    for bad in (lambda: scaled.encode(ws, x.t()), lambda: scaled.encode(ws, x.double()),
+                lambda: scaled.encode(ws, x, out=b), lambda: scaled.rms_norm(ws, x, x[0, :5]),
+                lambda: scaled.rms_norm(ws, x, residual=x.bfloat16()),
+                lambda: scaled.matmul(ws, a, b, out=out[:, :5]),
+                lambda: scaled.matmul(ws, a, b, dtype=torch.float64)):
+        with pytest.raises(ValueError):
+            bad()

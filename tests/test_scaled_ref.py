@@ -44,3 +44,33 @@ def test_entry_points_refuse_a_missing_workspace(autlib):
     assert autlib.aut_gemm_scaled(None, 0, 0, 0, None, 0, None, 0, None, 0, None, 0, 0, 0, 0,
                                   None, 0, None) == bad
     assert b"workspace" in autlib.aut_last_error()
+
+
+def test_tensor_calls_refuse_what_does_not_fit():
+    """scaled.* check their tensors before anything is launched."""
+    from accessor_universal_test_b200 import scaled
+
+    class Handle:  # a workspace's device is all the checks look at
+        device = 0
+
+    ws = Handle()
+    x = torch.zeros(4, 256)
+    with pytest.raises(ValueError, match="workspace on cuda:0"):
+        scaled.encode(ws, x)
+    with pytest.raises(ValueError, match="two dimensions"):
+        scaled.encode(ws, x[0])
+    with pytest.raises(ValueError, match="two dimensions"):
+        scaled.rms_norm(ws, x[0])
+    with pytest.raises(ValueError, match="block_rows"):
+        scaled.Scaled(4, 256, block_rows=2)
+    with pytest.raises(ValueError, match="code"):
+        scaled.Scaled(4, 256, code=7)
+    a, b = scaled.Scaled(4, 256), scaled.Scaled(300, 256, block_rows=128)
+    assert a.scales.shape == (2, 4) and b.scales.shape == (2, 3)
+    assert scaled.Scaled(3, 100).storage.shape == (3, 112)
+    with pytest.raises(ValueError, match="scales by rows"):
+        scaled.matmul(ws, b, b)
+    with pytest.raises(ValueError, match="columns"):
+        scaled.matmul(ws, a, scaled.Scaled(300, 128, block_rows=128))
+    with pytest.raises(ValueError, match="workspace on cuda:0"):
+        scaled.matmul(ws, a, b)
