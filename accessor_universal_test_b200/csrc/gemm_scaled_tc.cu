@@ -25,7 +25,10 @@ constexpr int kMaxDevices = 16;
 constexpr int kTileM = 128;
 // Blocks of k whose scales are brought at a time, and how many such batches
 // there is room for.
-constexpr int kScaleBatch = 4, kScaleSlots = 4;
+constexpr int kScaleBatch = 4, kScaleSlots = 2;
+// Results that do not go out in 16-byte stores are turned, 16 rows of 16 words at
+// a time, so that a warp writes whole lines of rows.
+constexpr int kTurnPitch = 17;
 // A load takes a few thousand cycles at most: a pair's pause for them once one
 // of its waits has given up (about half a millisecond).
 constexpr long long kPairDrainCycles = 1000000;
@@ -277,6 +280,38 @@ __device__ __forceinline__ void store_eight(const tile_params &p, uint64_t i, ui
   }
 }
 
+// W words (of one or two results of Size bytes) of each of a warp's 32 rows from
+// row i0 on, lane by lane a row, written by lines of rows.
+template <int Size, int W>
+__device__ __forceinline__ void store_turned(const tile_params &p, uint32_t *turn, int lane,
+                                             uint64_t i0, uint64_t j0, const uint32_t (&words)[W]) {
+  constexpr int kEach = 4 / Size; // results to a word
+  const gemm_params &g = p.g;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    __syncwarp();
+    if (lane / 16 == half) {
+#pragma unroll
+      for (int w = 0; w < W; ++w) turn[lane % 16 * kTurnPitch + w] = words[w];
+    }
+    __syncwarp();
+#pragma unroll
+    for (int at = 0; at < 16 * W; at += 32) {
+      const int r = (at + lane) / W, w = (at + lane) % W;
+      const uint64_t i = i0 + 16 * half + r, j = j0 + kEach * w;
+      const uint32_t word = turn[r * kTurnPitch + w];
+      if (i >= g.m || j >= g.n) continue;
+      unsigned char *to = static_cast<unsigned char *>(g.out) + (i * g.out_stride + j) * Size;
+      if (Size == 4 || (j + 1 < g.n && reinterpret_cast<uintptr_t>(to) % 4 == 0)) {
+        *reinterpret_cast<uint32_t *>(to) = word;
+      } else {
+        reinterpret_cast<uint16_t *>(to)[0] = static_cast<uint16_t>(word);
+        if (j + 1 < g.n) reinterpret_cast<uint16_t *>(to)[1] = static_cast<uint16_t>(word >> 16);
+      }
+    }
+  }
+}
+
 // Four neighbouring results.
 __device__ __forceinline__ void store_four(const tile_params &p, uint64_t i, uint64_t j,
                                            const float2 *v) {
@@ -309,7 +344,7 @@ template <int BN, bool Pair> struct tile_shape {
   static constexpr int kBRows = Pair ? BN / 2 : BN;
   static constexpr int kBBytes = kBRows * kBlock;
   static constexpr int kMostStages = 10;
-  static constexpr int kRingBytes = 208 * 1024;
+  static constexpr int kRingBytes = (BN >= 128 ? 200 : 208) * 1024;
   // Epilogue warps: four to a scheduler for the wide tiles, so that some read
   // tensor memory while others add (4096 x 8192 x 8192: 865 cycles a block of
   // k and tile where two to a scheduler took 962; the products alone, 513).
@@ -363,6 +398,7 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
   __shared__ __align__(8) uint64_t drained;
   // of both operands multiplied, for either side of the columns
   __shared__ float scales[shape::kSides][kScaleSlots][kScaleBatch][kTileM];
+  __shared__ uint32_t turn[shape::kEpilogueWarps][16 * kTurnPitch];
   __shared__ uint32_t tmem_base;
   __shared__ int gave_up_word;
   volatile int *gave_up = &gave_up_word;
@@ -637,11 +673,35 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
               make_float4(acc[c].x, acc[c].y, acc[c + 1].x, acc[c + 1].y);
         break;
       }
-      const uint64_t i = uint64_t{tm} * shape::kTileRows + rank * kTileM + row;
+      const uint64_t i0 = uint64_t{tm} * shape::kTileRows + rank * kTileM + warp % 4 * 32;
       const uint64_t j0 = uint64_t{tn} * BN + stripe * kColumns;
-      if (i < p.g.m) {
+      if (p.wide_out) {
+        if (i0 + lane < p.g.m) {
 #pragma unroll
-        for (int c = 0; c < kColumns; c += 8) store_eight(p, i, j0 + c, acc + c / 2);
+          for (int c = 0; c < kColumns; c += 8) store_eight(p, i0 + lane, j0 + c, acc + c / 2);
+        }
+      } else if (p.g.type == AUT_TYPE_FP32) {
+#pragma unroll
+        for (int c = 0; c < kColumns; c += 16) {
+          uint32_t words[16];
+#pragma unroll
+          for (int w = 0; w < 8; ++w) {
+            words[2 * w] = __float_as_uint(acc[c / 2 + w].x);
+            words[2 * w + 1] = __float_as_uint(acc[c / 2 + w].y);
+          }
+          store_turned<4>(p, turn[warp], lane, i0, j0 + c, words);
+        }
+      } else {
+        constexpr int kWords = kColumns < 32 ? 8 : 16;
+#pragma unroll
+        for (int c = 0; c < kColumns; c += 2 * kWords) {
+          uint32_t words[kWords];
+#pragma unroll
+          for (int w = 0; w < kWords; ++w)
+            words[w] = p.g.type == AUT_TYPE_BF16 ? pack_bf16(acc[c / 2 + w].x, acc[c / 2 + w].y)
+                                                 : pack_fp16(acc[c / 2 + w].x, acc[c / 2 + w].y);
+          store_turned<2>(p, turn[warp], lane, i0, j0 + c, words);
+        }
       }
     }
   }
