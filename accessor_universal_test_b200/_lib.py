@@ -143,6 +143,10 @@ class Workspace:
         check(lib.aut_workspace_create(device, C.byref(h)))
         self.handle = h
         self.device = device
+        # of the calls that a step of single tokens makes most often
+        self._encode_scaled = lib.aut_encode_scaled
+        self._rms_norm_scaled = lib.aut_rms_norm_scaled
+        self._gemm_scaled = lib.aut_gemm_scaled
         sm, mb = C.c_int32(), C.c_int32()
         check(lib.aut_workspace_info(h, C.byref(sm), C.byref(mb)))
         self.sm_count, self.max_blocks = sm.value, mb.value
@@ -197,28 +201,34 @@ class Workspace:
         """Values to 8-bit codes with a scale per block of block_rows x 128
         (strides in elements; the scale of row group R, column block b stands
         at scales[b * scale_stride + R])."""
-        check(load().aut_encode_scaled(self.handle, code, type, block_rows, values_ptr,
-                                       value_stride, rows, columns, codes_ptr, code_stride,
-                                       scales_ptr, scale_stride, stream))
+        status = self._encode_scaled(self.handle, code, type, block_rows, values_ptr,
+                                     value_stride, rows, columns, codes_ptr, code_stride,
+                                     scales_ptr, scale_stride, stream)
+        if status:
+            check(status)
 
     def rms_norm_scaled(self, code, type, x_ptr, x_stride, residual_ptr, residual_out_ptr,
                         residual_stride, weight_ptr, eps, rows, columns, codes_ptr, code_stride,
                         scales_ptr, scale_stride, stream=0) -> None:
         """Root-mean-square norm of x + residual, encoded with a scale per row
         and 128 columns; residual, residual_out and weight may be 0 (absent)."""
-        check(load().aut_rms_norm_scaled(self.handle, code, type, x_ptr, x_stride, residual_ptr,
-                                         residual_out_ptr, residual_stride, weight_ptr, eps,
-                                         rows, columns, codes_ptr, code_stride, scales_ptr,
-                                         scale_stride, stream))
+        status = self._rms_norm_scaled(self.handle, code, type, x_ptr, x_stride, residual_ptr,
+                                       residual_out_ptr, residual_stride, weight_ptr, eps, rows,
+                                       columns, codes_ptr, code_stride, scales_ptr, scale_stride,
+                                       stream)
+        if status:
+            check(status)
 
     def gemm_scaled(self, a_code, b_code, type, a_ptr, a_stride, a_scales_ptr, a_scale_stride,
                     b_ptr, b_stride, b_scales_ptr, b_scale_stride, m, n, k, out_ptr, out_stride,
                     stream=0) -> None:
         """out[m, n] = a[m, k] times b[n, k] transposed, both block-scaled
         codes: a with a scale per row, b with one per 128 rows."""
-        check(load().aut_gemm_scaled(self.handle, a_code, b_code, type, a_ptr, a_stride,
-                                     a_scales_ptr, a_scale_stride, b_ptr, b_stride, b_scales_ptr,
-                                     b_scale_stride, m, n, k, out_ptr, out_stride, stream))
+        status = self._gemm_scaled(self.handle, a_code, b_code, type, a_ptr, a_stride,
+                                   a_scales_ptr, a_scale_stride, b_ptr, b_stride, b_scales_ptr,
+                                   b_scale_stride, m, n, k, out_ptr, out_stride, stream)
+        if status:
+            check(status)
 
 
 def generate_dot_v1(family: int, seed: int, parameter: int, vector_id: int, count: int,

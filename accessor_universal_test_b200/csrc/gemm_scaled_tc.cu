@@ -25,7 +25,7 @@ constexpr int kMaxDevices = 16;
 constexpr int kTileM = 128;
 // Blocks of k whose scales are brought at a time, and how many such batches
 // there is room for.
-constexpr int kScaleBatch = 4, kScaleSlots = 2;
+constexpr int kScaleBatch = 4, kScaleSlots = 4;
 // Results that do not go out in 16-byte stores are turned, 16 rows of 16 words at
 // a time, so that a warp writes whole lines of rows.
 constexpr int kTurnPitch = 17;
@@ -344,7 +344,7 @@ template <int BN, bool Pair> struct tile_shape {
   static constexpr int kBRows = Pair ? BN / 2 : BN;
   static constexpr int kBBytes = kBRows * kBlock;
   static constexpr int kMostStages = 10;
-  static constexpr int kRingBytes = (BN >= 128 ? 200 : 208) * 1024;
+  static constexpr int kRingBytes = (BN == 256 ? 192 : BN == 128 ? 200 : 204) * 1024;
   // Epilogue warps: four to a scheduler for the wide tiles, so that some read
   // tensor memory while others add (4096 x 8192 x 8192: 865 cycles a block of
   // k and tile where two to a scheduler took 962; the products alone, 513).
@@ -379,8 +379,10 @@ __device__ __forceinline__ void tile_at(uint32_t tile, const tile_params &p, uin
 
 // Split: the blocks of a cluster share a tile's blocks of k, where there are
 // fewer tiles than SMs; each has one tile, and their sums are joined over
-// distributed shared memory in the order of the parts.
-template <int BN, bool Pair, bool Split>
+// distributed shared memory in the order of the parts.  Turn: rows of out do not
+// start on 16 bytes; a kernel of its own, whose registers the others do without
+// (4096 x 8192 x 8192: 256 against 279 us).
+template <int BN, bool Pair, bool Split, bool Turn>
 __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
     tiles_kernel(const __grid_constant__ CUtensorMap map_a,
                  const __grid_constant__ CUtensorMap map_b, const tile_params p) {
@@ -398,7 +400,7 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
   __shared__ __align__(8) uint64_t drained;
   // of both operands multiplied, for either side of the columns
   __shared__ float scales[shape::kSides][kScaleSlots][kScaleBatch][kTileM];
-  __shared__ uint32_t turn[shape::kEpilogueWarps][16 * kTurnPitch];
+  __shared__ uint32_t turn[Turn ? shape::kEpilogueWarps : 1][16 * kTurnPitch];
   __shared__ uint32_t tmem_base;
   __shared__ int gave_up_word;
   volatile int *gave_up = &gave_up_word;
@@ -675,7 +677,7 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
       }
       const uint64_t i0 = uint64_t{tm} * shape::kTileRows + rank * kTileM + warp % 4 * 32;
       const uint64_t j0 = uint64_t{tn} * BN + stripe * kColumns;
-      if (p.wide_out) {
+      if constexpr (!Turn) {
         if (i0 + lane < p.g.m) {
 #pragma unroll
           for (int c = 0; c < kColumns; c += 8) store_eight(p, i0 + lane, j0 + c, acc + c / 2);
@@ -805,11 +807,11 @@ aut_status make_map(CUtensorMap *map, const uint8_t *codes, uint64_t rows, uint6
   return AUT_OK;
 }
 
-template <int BN, bool Pair, bool Split>
-aut_status launch_tiles(aut_workspace *ws, tile_params p, int a_code, int b_code,
+template <int BN, bool Pair, bool Split, bool Turn>
+aut_status launch_kind(aut_workspace *ws, tile_params p, int a_code, int b_code,
                         cudaStream_t stream) {
   using shape = tile_shape<BN, Pair>;
-  auto kernel = tiles_kernel<BN, Pair, Split>;
+  auto kernel = tiles_kernel<BN, Pair, Split, Turn>;
   CUtensorMap map_a, map_b;
   // rows of a tile beyond a's are not even filled with zeros: what the products
   // make of them is not stored
@@ -876,6 +878,15 @@ aut_status launch_tiles(aut_workspace *ws, tile_params p, int a_code, int b_code
   return AUT_OK;
 }
 
+template <int BN, bool Pair>
+aut_status launch_tiles(aut_workspace *ws, const tile_params &p, int a_code, int b_code,
+                        cudaStream_t stream) {
+  if constexpr (!Pair)
+    if (p.parts > 1) return launch_kind<BN, Pair, true, false>(ws, p, a_code, b_code, stream);
+  return p.wide_out ? launch_kind<BN, Pair, false, false>(ws, p, a_code, b_code, stream)
+                    : launch_kind<BN, Pair, false, true>(ws, p, a_code, b_code, stream);
+}
+
 } // namespace
 
 aut_status gemm_tiles(aut_workspace *ws, const gemm_params &g, int a_code, int b_code,
@@ -915,18 +926,11 @@ aut_status gemm_tiles(aut_workspace *ws, const gemm_params &g, int a_code, int b
       if (t < best) best = t, columns = kind.columns, p.parts = parts;
     }
   }
-  const bool split = p.parts > 1;
   switch (columns) {
-  case 32:
-    return split ? launch_tiles<32, false, true>(ws, p, a_code, b_code, stream)
-                 : launch_tiles<32, false, false>(ws, p, a_code, b_code, stream);
-  case 64:
-    return split ? launch_tiles<64, false, true>(ws, p, a_code, b_code, stream)
-                 : launch_tiles<64, false, false>(ws, p, a_code, b_code, stream);
-  case 128:
-    return split ? launch_tiles<128, false, true>(ws, p, a_code, b_code, stream)
-                 : launch_tiles<128, false, false>(ws, p, a_code, b_code, stream);
-  default: return launch_tiles<256, true, false>(ws, p, a_code, b_code, stream);
+  case 32: return launch_tiles<32, false>(ws, p, a_code, b_code, stream);
+  case 64: return launch_tiles<64, false>(ws, p, a_code, b_code, stream);
+  case 128: return launch_tiles<128, false>(ws, p, a_code, b_code, stream);
+  default: return launch_tiles<256, true>(ws, p, a_code, b_code, stream);
   }
 }
 

@@ -833,14 +833,15 @@ static uint64_t size_of_type(int32_t type) { return type == AUT_TYPE_FP32 ? 4 : 
 
 static aut_status check_matrix(const char *name, const void *pointer, uint64_t rows,
                                uint64_t columns, uint64_t stride, uint64_t size) {
-  const std::string what(name);
-  if (pointer == nullptr) return fail(AUT_ERR_INVALID_ARGUMENT, what + " is NULL");
+  if (pointer == nullptr) return fail(AUT_ERR_INVALID_ARGUMENT, std::string(name) + " is NULL");
   if (reinterpret_cast<uintptr_t>(pointer) % size != 0)
-    return fail(AUT_ERR_INVALID_ARGUMENT, what + " is not aligned to its elements");
+    return fail(AUT_ERR_INVALID_ARGUMENT,
+                std::string(name) + " is not aligned to its elements");
   if (rows > 1 && stride < columns)
-    return fail(AUT_ERR_INVALID_ARGUMENT, what + ": stride smaller than one row");
+    return fail(AUT_ERR_INVALID_ARGUMENT,
+                std::string(name) + ": stride smaller than one row");
   if (rows > 1 && stride > (uint64_t{1} << 53) / size / (rows - 1))
-    return fail(AUT_ERR_TOO_LARGE, what + ": matrix larger than 2^53 bytes");
+    return fail(AUT_ERR_TOO_LARGE, std::string(name) + ": matrix larger than 2^53 bytes");
   return AUT_OK;
 }
 
