@@ -5,6 +5,7 @@
 #include "scaled_device.cuh"
 
 #include <algorithm>
+#include <atomic>
 
 namespace aut::scaled {
 namespace {
@@ -123,10 +124,15 @@ __device__ __forceinline__ void store_chunk(T *row, uint32_t chunk, int lane, ui
   if constexpr (Vec) {
     if (c0 < columns) store_eight(row + c0, v);
   } else {
+    T *to = row + c0;
+    if (chunk * 256 + 256 <= columns) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c0 + 32 * j < columns)
-        row[c0 + 32 * j] = narrow<T>(j % 2 == 0 ? v[j / 2].x : v[j / 2].y);
+      for (int j = 0; j < 8; ++j) to[32 * j] = narrow<T>(j % 2 == 0 ? v[j / 2].x : v[j / 2].y);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c0 + 32 * j < columns) to[32 * j] = narrow<T>(j % 2 == 0 ? v[j / 2].x : v[j / 2].y);
+    }
   }
 }
 
@@ -163,7 +169,7 @@ __device__ __forceinline__ void encode_chunk(float2 (&v)[4], uint32_t chunk, int
     m[0] = largest_of(v[0], v[1]), m[1] = largest_of(v[2], v[3]);
     if (Vec) m[0] = fmaxf(m[0], m[1]);
   }
-  uint32_t codes[2];
+  uint32_t codes[4]; // two each
   block_scale s;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -173,16 +179,28 @@ __device__ __forceinline__ void encode_chunk(float2 (&v)[4], uint32_t chunk, int
       if ((Vec ? lane % 16 : lane) == 0 && block * kBlock < columns)
         scales[block * scale_stride] = s.scale;
     }
-    codes[h] = four_codes<Code>(quotient(v[2 * h], s), quotient(v[2 * h + 1], s));
+#pragma unroll
+    for (int j = 2 * h; j < 2 * h + 2; ++j) {
+      const float2 q = quotient(v[j], s);
+      codes[j] = codes_of<Code>(q.x, q.y);
+    }
   }
   const uint32_t c0 = column_of<Vec>(chunk, lane, 0);
   if constexpr (Vec) {
-    if (c0 < columns) *reinterpret_cast<uint2 *>(row + c0) = make_uint2(codes[0], codes[1]);
+    if (c0 < columns)
+      *reinterpret_cast<uint2 *>(row + c0) = make_uint2(__byte_perm(codes[0], codes[1], 0x5410),
+                                                        __byte_perm(codes[2], codes[3], 0x5410));
   } else {
+    uint8_t *to = row + c0;
+    if (chunk * 256 + 256 <= columns) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c0 + 32 * j < columns)
-        row[c0 + 32 * j] = static_cast<uint8_t>(codes[j / 4] >> (8 * (j % 4)));
+      for (int j = 0; j < 8; ++j) to[32 * j] = static_cast<uint8_t>(codes[j / 2] >> (8 * (j % 2)));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c0 + 32 * j < columns)
+          to[32 * j] = static_cast<uint8_t>(codes[j / 2] >> (8 * (j % 2)));
+    }
   }
 }
 
@@ -379,23 +397,23 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// Rows by Threads threads each, which hold a row in registers (FP32 h, Chunks
-// times eight values a thread), so x and the residual are read once; the
+// Rows by up to Threads threads each, which hold a row in registers (FP32 h,
+// Chunks times eight values a thread), so x and the residual are read once; the
 // weight stays in registers over the rows of a block.  The next row's values
 // are loaded before this one's are summed and encoded.  Threads = 32: four
 // rows to a block of 128.
 template <int Type, int Code, bool Vec, int Threads, int Chunks>
 __global__ void __launch_bounds__(Threads < 128 ? 128 : Threads,
-                                  65536 / (Threads < 512 ? 80 : 64) /
+                                  65536 / (Threads < 256 ? 48 : Threads < 512 ? 80 : 64) /
                                       (Threads < 128 ? 128 : Threads))
     norm_kernel(const norm_params p) {
   using T = element_t<Type>;
-  constexpr int kWarps = Threads / 32;
-  __shared__ float part[2][kWarps];
+  __shared__ float part[2][Threads / 32];
   aut::dev::pdl_wait();
   aut::dev::pdl_release();
   const int lane = threadIdx.x & 31;
   const int warp = Threads == 32 ? 0 : threadIdx.x / 32;
+  const int warps = Threads == 32 ? 1 : blockDim.x / 32;
   const uint64_t rows_a_block = Threads == 32 ? 4 : 1;
   const uint64_t step = gridDim.x * rows_a_block;
   uint64_t row = blockIdx.x * rows_a_block + (Threads == 32 ? threadIdx.x / 32 : 0);
@@ -407,14 +425,14 @@ __global__ void __launch_bounds__(Threads < 128 ? 128 : Threads,
   raw_chunk<T> next[Chunks], more[Chunks], weight[Chunks];
 #pragma unroll
   for (int i = 0; i < Chunks; ++i) {
-    next[i] = load_raw<Vec>(x, i * kWarps + warp, lane, columns);
+    next[i] = load_raw<Vec>(x, i * warps + warp, lane, columns);
     if (p.residual != nullptr)
-      more[i] = load_raw<Vec>(residual, i * kWarps + warp, lane, columns);
+      more[i] = load_raw<Vec>(residual, i * warps + warp, lane, columns);
   }
 #pragma unroll
   for (int i = 0; i < Chunks; ++i)
     if (p.weight != nullptr)
-      weight[i] = load_raw<Vec>(static_cast<const T *>(p.weight), i * kWarps + warp, lane, columns);
+      weight[i] = load_raw<Vec>(static_cast<const T *>(p.weight), i * warps + warp, lane, columns);
   for (int turn = 0; row < p.e.rows; row += step, turn ^= 1) {
     float2 h[Chunks][4], squares = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -432,9 +450,9 @@ __global__ void __launch_bounds__(Threads < 128 ? 128 : Threads,
       residual += step * p.residual_stride;
 #pragma unroll
       for (int i = 0; i < Chunks; ++i) {
-        next[i] = load_raw<Vec>(x, i * kWarps + warp, lane, columns);
+        next[i] = load_raw<Vec>(x, i * warps + warp, lane, columns);
         if (p.residual != nullptr)
-          more[i] = load_raw<Vec>(residual, i * kWarps + warp, lane, columns);
+          more[i] = load_raw<Vec>(residual, i * warps + warp, lane, columns);
       }
     }
 #pragma unroll
@@ -446,12 +464,12 @@ __global__ void __launch_bounds__(Threads < 128 ? 128 : Threads,
       // two sets of sums: no warp is more than one row ahead of another
       if (lane == 0) part[turn][warp] = sum;
       __syncthreads();
-      sum = warp_sum(lane < kWarps ? part[turn][lane] : 0.0f);
+      sum = warp_sum(lane < warps ? part[turn][lane] : 0.0f);
     }
     const float r = rsqrtf(sum / mean_of + p.eps);
 #pragma unroll
     for (int i = 0; i < Chunks; ++i) {
-      const uint32_t chunk = i * kWarps + warp;
+      const uint32_t chunk = i * warps + warp;
       if (chunk * 256 >= columns) break;
       if (p.residual_out != nullptr)
         store_chunk<Vec>(static_cast<T *>(p.residual_out) + row * p.residual_stride, chunk, lane,
@@ -597,25 +615,38 @@ aut_status encode_typed(aut_workspace *ws, int32_t block_rows, const encode_para
              : encode_by_tiles<Type, Code, false>(ws, p, stream);
 }
 
-template <int Type, int Code, bool Vec, int Threads>
+template <int Type, int Code, bool Vec, int Threads, int Chunks>
 aut_status norm_launch(aut_workspace *ws, const norm_params &p, cudaStream_t stream) {
-  constexpr int kBlockThreads = Threads < 128 ? 128 : Threads;
-  auto kernel = norm_kernel<Type, Code, Vec, Threads, 2>;
-  static const int resident = resident_blocks(kernel, kBlockThreads);
+  auto kernel = norm_kernel<Type, Code, Vec, Threads, Chunks>;
+  // as many warps as hold the row
+  const uint64_t columns = 256 * Chunks;
+  const int warps = Threads == 32 ? 4 : static_cast<int>((p.e.columns + columns - 1) / columns);
+  static std::atomic<int> resident[33];
+  int n = resident[warps].load(std::memory_order_relaxed);
+  if (n == 0)
+    resident[warps].store(n = resident_blocks(kernel, 32 * warps), std::memory_order_relaxed);
   const uint64_t blocks = Threads == 32 ? (p.e.rows + 3) / 4 : p.e.rows;
-  return launch(kernel, std::min(blocks, static_cast<uint64_t>(resident * ws->sm_count)),
-                kBlockThreads, p, stream);
+  return launch(kernel, std::min(blocks, static_cast<uint64_t>(n * ws->sm_count)), 32 * warps, p,
+                stream);
 }
 
-// The fewest threads that hold a row with 16 values each.
+// Sixteen values a thread, or eight: where that is one warp or few (4096 x 640
+// BF16: 5.0 against 5.8 us), for values of 32 bits, which sixteen leave no
+// registers for the next row (4096 x 5001: 47 against 59 us), and where there
+// is less than a row for every SM, so that the time of one row counts (1 x 4096:
+// 1.8 against 2.0 us).  Elsewhere sixteen keep more rows under way (4096 x 5000
+// BF16: 27 against 31 us).
 template <int Type, int Code, bool Vec>
 aut_status norm_rows(aut_workspace *ws, const norm_params &p, cudaStream_t stream) {
   const uint64_t columns = p.e.columns;
-  if (columns <= 512) return norm_launch<Type, Code, Vec, 32>(ws, p, stream);
-  if (columns <= 2048) return norm_launch<Type, Code, Vec, 128>(ws, p, stream);
-  if (columns <= 4096) return norm_launch<Type, Code, Vec, 256>(ws, p, stream);
-  if (columns <= 8192) return norm_launch<Type, Code, Vec, 512>(ws, p, stream);
-  return norm_launch<Type, Code, Vec, 1024>(ws, p, stream);
+  if (columns <= 256) return norm_launch<Type, Code, Vec, 32, 1>(ws, p, stream);
+  if (columns <= 1024) return norm_launch<Type, Code, Vec, 128, 1>(ws, p, stream);
+  if (columns <= 8192 &&
+      (Type == AUT_TYPE_FP32 || p.e.rows <= static_cast<uint64_t>(ws->sm_count)))
+    return norm_launch<Type, Code, Vec, 1024, 1>(ws, p, stream);
+  if (columns <= 4096) return norm_launch<Type, Code, Vec, 256, 2>(ws, p, stream);
+  if (columns <= 8192) return norm_launch<Type, Code, Vec, 512, 2>(ws, p, stream);
+  return norm_launch<Type, Code, Vec, 1024, 2>(ws, p, stream);
 }
 
 template <int Type, int Code>
