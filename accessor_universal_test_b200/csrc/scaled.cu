@@ -263,10 +263,11 @@ template <class T> __device__ __forceinline__ void widen_four(const raw_four<T> 
   v[0] = widen_pair(r.w[0], T{}), v[1] = widen_pair(r.w[1], T{});
 }
 
-// column: the lane's first; what is beyond the matrix reads as zero.
+// column: the lane's first; what is beyond the matrix reads as zero.  whole: the
+// tile lies in the matrix.
 template <bool Vec, class T>
-__device__ __forceinline__ raw_four<T> load_four(const T *row, bool has_row, uint32_t column,
-                                                 uint32_t columns) {
+__device__ __forceinline__ raw_four<T> load_four(const T *row, bool whole, bool has_row,
+                                                 uint32_t column, uint32_t columns) {
   raw_four<T> r;
   if constexpr (Vec) {
     const bool has = has_row && column < columns;
@@ -281,9 +282,14 @@ __device__ __forceinline__ raw_four<T> load_four(const T *row, bool has_row, uin
     using word = typename raw_word<sizeof(T)>::type;
     const word *x = reinterpret_cast<const word *>(row + column);
     uint32_t bits[4];
+    if (whole) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      bits[j] = has_row && column + 32 * j < columns ? x[32 * j] : word{0};
+      for (int j = 0; j < 4; ++j) bits[j] = x[32 * j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        bits[j] = has_row && column + 32 * j < columns ? x[32 * j] : word{0};
+    }
 #pragma unroll
     for (int i = 0; i < static_cast<int>(sizeof(T)); ++i)
       r.w[i] = sizeof(T) == 4 ? bits[i] : bits[2 * i % 4] | bits[(2 * i + 1) % 4] << 16;
@@ -310,12 +316,16 @@ __global__ void __launch_bounds__(tile_of<element_t<Type>>::kThreads,
   uint32_t block = blockIdx.x % blocks;
   const uint32_t lane_column = Vec ? lane * 4 : lane;
   raw_four<T> next[tile::kRows];
+  auto is_whole = [&](uint64_t group, uint32_t block) {
+    return (group + 1) * kBlock <= p.rows && (block + 1) * kBlock <= columns;
+  };
   auto load = [&] {
     const uint64_t first = group * kBlock + warp;
     const T *x = static_cast<const T *>(p.x) + first * p.x_stride;
+    const bool whole = is_whole(group, block);
 #pragma unroll
     for (int r = 0; r < tile::kRows; ++r)
-      next[r] = load_four<Vec>(x + r * tile::kWarps * p.x_stride,
+      next[r] = load_four<Vec>(x + r * tile::kWarps * p.x_stride, whole,
                                first + r * tile::kWarps < p.rows, block * kBlock + lane_column,
                                columns);
   };
@@ -367,6 +377,7 @@ __global__ void __launch_bounds__(tile_of<element_t<Type>>::kThreads,
     const uint64_t first = group_now * kBlock + warp;
     const uint32_t column = block_now * kBlock + lane_column;
     uint8_t *to = p.codes + first * p.code_stride + column;
+    const bool whole = is_whole(group_now, block_now);
 #pragma unroll
     for (int r = 0; r < tile::kRows; ++r, to += tile::kWarps * p.code_stride) {
       float2 v[2];
@@ -380,6 +391,9 @@ __global__ void __launch_bounds__(tile_of<element_t<Type>>::kThreads,
       const bool has_row = first + r * tile::kWarps < p.rows;
       if constexpr (Vec) {
         if (has_row && column < columns) *reinterpret_cast<uint32_t *>(to) = codes;
+      } else if (whole) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) to[32 * j] = static_cast<uint8_t>(codes >> (8 * j));
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
