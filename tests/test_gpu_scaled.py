@@ -391,6 +391,40 @@ def test_gemm_keeps_nan_and_infinity_in_their_rows(ws, m):
     np.testing.assert_array_equal(got[np.ix_(rows, columns)], clean[np.ix_(rows, columns)])
 
 
+@pytest.mark.parametrize("m", [1, 20, 33, 64, 65, 130])
+@pytest.mark.parametrize("k", [1, 2, 3, 5, 126, 127, 129, 131, 255, 383, 640])
+def test_gemm_rows_on_any_boundary(ws, m, k):
+    n, a_code, b_code = 140, (m + k) % 2, (m // 2 + k) % 2
+    a, sa = operand(m, k, a_code, 1, m)
+    b, sb = operand(n, k, b_code, 128, k)
+    # rows on every offset from 4 bytes on both sides; NaN codes around the rows
+    for layout in (dict(a_stride=k + 1 - k % 2, b_stride=k + 3 - k % 2, a_offset=1),
+                   dict(a_stride=up16(k) + 2, b_stride=up16(k) + 4, b_offset=3),
+                   dict(a_stride=up16(k), b_stride=up16(k) + 7)):
+        got = run_gemm(ws, a, sa, b, sb, a_code, b_code, FP32, **layout)
+        check_gemm(got, a, sa, b, sb, a_code, b_code, FP32)
+
+
+@pytest.mark.parametrize("m", [10, 70])
+def test_gemm_keeps_nan_and_infinity_in_their_rows_on_any_boundary(ws, m):
+    n, k = 150, 403
+    a, sa = operand(m, k, ref.E5M2, 1, 3)
+    b, sb = operand(n, k, ref.E4M3, 128, 4)
+    layout = dict(a_stride=k, b_stride=k, a_offset=1)
+    clean = run_gemm(ws, a, sa, b, sb, ref.E5M2, ref.E4M3, FP32, **layout)
+    a[1, 402], b[5, 0] = 0x7f, 0xff  # NaN codes
+    b[b & 0x7f == 0] = 0x38  # no zeros against infinity
+    clean_again = run_gemm(ws, a, sa, b, sb, ref.E5M2, ref.E4M3, FP32, **layout)
+    a[2, 3] = 0x7c  # infinity
+    got = run_gemm(ws, a, sa, b, sb, ref.E5M2, ref.E4M3, FP32, **layout)
+    assert np.isfinite(clean).all()
+    assert np.isnan(got[1]).all() and np.isnan(got[:, 5]).all()
+    assert not np.isfinite(got[2]).any()
+    rows, columns = [i for i in range(m) if i not in (1, 2)], [j for j in range(n) if j != 5]
+    np.testing.assert_array_equal(got[np.ix_(rows, columns)], clean_again[np.ix_(rows, columns)])
+    assert np.isfinite(got[np.ix_(rows, columns)]).all()
+
+
 @pytest.mark.parametrize("m", [2, 30, 200])
 def test_gemm_zero_rows_and_repeats(ws, m):
     a, sa = operand(m, 1024, ref.E4M3, 1, 3)
