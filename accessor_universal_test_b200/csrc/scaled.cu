@@ -209,6 +209,11 @@ __device__ __forceinline__ void encode_chunk(float2 (&v)[4], uint32_t chunk, int
 // rows, a warp two rows of a group; the next group's values are loaded before
 // this one's are encoded, so loads are under way all the time.  The rows of a
 // group are neighbours: the scales of one column block fill whole lines.
+// Bound by memory, with the schedulers busy two thirds of the time (the search
+// for the maximum, the scale and the conversions).  Measured, copy bandwidth
+// 6.55 TB/s: 4096 x 8192 BF16 18.1 us (5.6 TB/s), FP32 26.4 (6.4); 4096 x 5001 FP32
+// 18.6 (5.6), FP16 19.9 (3.1: eight loads and eight stores of a lane for
+// one of each where rows start on 16 bytes).
 constexpr int kEncodeRows = 16;
 
 template <int Type, int Code, bool Vec>
@@ -246,7 +251,9 @@ __global__ void __launch_bounds__(256) encode_rows_kernel(const encode_params p)
 // A block holds a tile in registers (16 a thread: 32 values of 16 bits, 16 of
 // 32), so the tile is read once, and loads its next one before it encodes this
 // one.  Vec: lane l holds the columns 4 l .., a multiple of 4 in all; else
-// l + 32 j (see above).
+// l + 32 j (see above).  Measured: 8192 x 8192 FP32 51.3 us (6.5 TB/s), 8192 x 5120
+// BF16 24.6 (5.1), 8191 x 5001 FP32 35.4 (5.8), FP16 40.4 (3.0; with a test of row
+// and column at each value of every tile 51.7).
 template <class T> struct tile_of {
   static constexpr int kThreads = sizeof(T) == 4 ? 1024 : 512;
   static constexpr int kWarps = kThreads / 32;
@@ -415,7 +422,11 @@ __device__ __forceinline__ float warp_sum(float v) {
 // Chunks times eight values a thread), so x and the residual are read once; the
 // weight stays in registers over the rows of a block.  The next row's values
 // are loaded before this one's are summed and encoded.  Threads = 32: four
-// rows to a block of 128.
+// rows to a block of 128.  Bound by memory; one barrier a row, which the other
+// blocks of the SM fill.  Measured with a residual in place: 4096 x 8192 BF16 39.9 us
+// (5.9 TB/s), 4096 x 4096 FP32 35.6 (6.1), 4096 x 5001 FP32 47.3 (5.6), BF16 55.2 (2.6:
+// the same count of instructions as FP32 for half the bytes, and stores of 64
+// bytes that begin and end within a sector), 1 x 4096 BF16 1.7.
 template <int Type, int Code, bool Vec, int Threads, int Chunks>
 __global__ void __launch_bounds__(Threads < 128 ? 128 : Threads,
                                   65536 / (Threads < 256 ? 48 : Threads < 512 ? 80 : 64) /

@@ -21,9 +21,6 @@ template <> struct element<AUT_TYPE_BF16> { using type = __nv_bfloat16; };
 template <> struct element<AUT_TYPE_FP16> { using type = __half; };
 template <int Type> using element_t = typename element<Type>::type;
 
-__device__ __forceinline__ float widen(float v) { return v; }
-__device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float widen(__half v) { return __half2float(v); }
 template <class T> __device__ __forceinline__ T narrow(float v);
 template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) {
