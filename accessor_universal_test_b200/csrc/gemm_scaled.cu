@@ -22,6 +22,22 @@ __device__ __forceinline__ int offset_in_word(const uint8_t *row) {
   return static_cast<int>(reinterpret_cast<uintptr_t>(row) & 3);
 }
 
+// The last codes of a row, byte by byte: a kernel whose registers are full
+// comes here once a row at most.
+__device__ __forceinline__ uint4 load_last(const uint8_t *row, uint64_t c, uint64_t k) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w[i] = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint64_t at = c + 4 * i + j;
+      if (at < k) w[i] |= uint32_t{row[at]} << (8 * j);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // Sixteen codes of a row of any alignment from column c, a multiple of 16, on.
 __device__ __forceinline__ uint4 load_codes(const uint8_t *row, uint64_t c, uint64_t k) {
   const int s = offset_in_word(row);
@@ -417,10 +433,10 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(const gemm_params p) {
           for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-              if (has_b[r][h]) u[i][r][h][half] = load_codes(b[r][h] - 32 * t, c, p.k);
+              if (has_b[r][h]) u[i][r][h][half] = load_last(b[r][h] - 32 * t, c, p.k);
 #pragma unroll
           for (int x = 0; x < T; ++x)
-            if (has_a[x]) w[i][x][half] = load_codes(a[x] - 32 * t, c, p.k);
+            if (has_a[x]) w[i][x][half] = load_last(a[x] - 32 * t, c, p.k);
         }
       }
 #pragma unroll
