@@ -22,22 +22,6 @@ __device__ __forceinline__ int offset_in_word(const uint8_t *row) {
   return static_cast<int>(reinterpret_cast<uintptr_t>(row) & 3);
 }
 
-// The last codes of a row, byte by byte: a kernel whose registers are full
-// comes here once a row at most.
-__device__ __forceinline__ uint4 load_last(const uint8_t *row, uint64_t c, uint64_t k) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    w[i] = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint64_t at = c + 4 * i + j;
-      if (at < k) w[i] |= uint32_t{row[at]} << (8 * j);
-    }
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 // Sixteen codes of a row of any alignment from column c, a multiple of 16, on.
 __device__ __forceinline__ uint4 load_codes(const uint8_t *row, uint64_t c, uint64_t k) {
   const int s = offset_in_word(row);
@@ -48,6 +32,21 @@ __device__ __forceinline__ uint4 load_codes(const uint8_t *row, uint64_t c, uint
   w[4] = s == 0 ? 0u : load_word(row, first + 16, end);
   return make_uint4(__funnelshift_r(w[0], w[1], 8 * s), __funnelshift_r(w[1], w[2], 8 * s),
                     __funnelshift_r(w[2], w[3], 8 * s), __funnelshift_r(w[3], w[4], 8 * s));
+}
+
+// The same of a row on a 16-byte boundary; what its end cuts is read byte by byte
+// in a loop, which takes few registers (1 x 4096 x 4000: 5.1 us; 8.4 with all bytes
+// at once, which spills).
+__device__ __forceinline__ uint4 load_end(const uint8_t *row, uint64_t c, uint64_t k) {
+  if (c + 16 <= k) return __ldg(reinterpret_cast<const uint4 *>(row + c));
+  uint64_t lo = 0, hi = 0;
+#pragma unroll 1
+  for (uint64_t at = k; at-- > c;) {
+    hi = hi << 8 | lo >> 56;
+    lo = lo << 8 | row[at];
+  }
+  return make_uint4(static_cast<uint32_t>(lo), static_cast<uint32_t>(lo >> 32),
+                    static_cast<uint32_t>(hi), static_cast<uint32_t>(hi >> 32));
 }
 
 // d += a (16 x 32) * b (32 x 8), FP32 sums.  LeftCode and RightCode name the
@@ -83,6 +82,31 @@ __device__ __forceinline__ void join_warps(const gemm_params &p, const float (&s
     for (int w = 0; w < 8; ++w) s += sums[w][r][c];
     if (n0 + r < p.n && m0 + c < p.m) store_out(p, m0 + c, n0 + r, s);
   }
+}
+
+// The same over the thread blocks of a cluster, in rank order: each stores a
+// share of the sums.
+template <int Rows, int Columns, int Parts>
+__device__ __forceinline__ void join_cluster(const gemm_params &p,
+                                             const float (&sums)[8][Rows][Columns], uint64_t n0,
+                                             uint32_t rank) {
+  __shared__ float joined[Rows * Columns];
+  for (int at = threadIdx.x; at < Rows * Columns; at += 256) {
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) s += sums[w][at % Rows][at / Rows];
+    joined[at] = s;
+  }
+  cluster_sync();
+  constexpr uint32_t share = Rows * Columns / Parts;
+  for (uint32_t i = threadIdx.x; i < share; i += 256) {
+    const uint32_t at = rank * share + i;
+    float s = 0.0f;
+#pragma unroll
+    for (uint32_t q = 0; q < Parts; ++q) s += cluster_load(&joined[at], q);
+    if (n0 + at % Rows < p.n && at / Rows < p.m) store_out(p, at / Rows, n0 + at % Rows, s);
+  }
+  cluster_sync(); // no block leaves before the others have read its sums
 }
 
 // ---- any alignment, few rows of a ----------------------------------------------------
@@ -321,9 +345,9 @@ __global__ void __launch_bounds__(kAnyThreads, 2) any_tiles_kernel(const gemm_pa
 
 // ---- few rows of a -----------------------------------------------------------------
 // The product reads b once and computes little: what counts is how many bytes
-// are under way.  A thread block computes 16 R rows of b against all rows of a
-// (8 T); its eight warps share the blocks of k, kAhead at a time, all of whose
-// loads are issued before the first product.  Measured (m x n x k, GB/s of
+// are under way.  A thread block computes 16 rows of b against all rows of a
+// (8 T); its eight warps, or those of a cluster of Parts blocks, share the blocks
+// of k, kAhead at a time, all of whose loads are issued before the first product.  Measured (m x n x k, GB/s of
 // codes): 1 x 4096 x 4096 with kAhead 1, 2, 3, 4: 3387, 3640, 2963, 2729;
 // 8 x 8192 x 8192: 3763, 4364, 4063, 4004 (registers: fewer blocks to an SM);
 // keeping the next kAhead blocks' loads under way behind each product: 4181.
@@ -349,154 +373,153 @@ __device__ __forceinline__ void stream_load(const uint8_t *p, uint4 &v, uint4 &w
   }
 }
 
-template <int ACode, int BCode, int R, int T, bool Wide>
+template <int ACode, int BCode, int T, bool Wide, int Parts>
 __global__ void __launch_bounds__(256, 2) stream_kernel(const gemm_params p) {
   constexpr int kAhead = T == 1 ? 2 : 1;
-  __shared__ float sums[8][16 * R][8 * T];
+  __shared__ float sums[8][16][8 * T];
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
   const int g = lane >> 2, t = lane & 3;
-  const uint64_t n0 = uint64_t{blockIdx.x} * (16 * R);
+  const uint32_t rank = blockIdx.x % Parts;
+  const uint64_t n0 = uint64_t{blockIdx.x / Parts} * 16;
+  // this one of the warps that share the blocks of k
+  constexpr uint32_t sharers = 8 * Parts;
+  const uint32_t own = rank * 8 + warp;
   // A hint for the second-level cache, which is coherent, so it may come before
   // the kernels before this one have ended (1 x 4096 x 4096: 6.1 -> 4.6 us with
-  // launches one behind the other): each lane's line of its row pairs' blocks
-  // warp, warp + 8, + 16 and + 24.
-  const uint64_t ahead = (uint64_t{static_cast<uint32_t>(warp)} + 8 * t) * kBlock;
+  // launches one behind the other): each lane's line of its two rows' blocks
+  // own, own + sharers and so on.
+  const uint64_t ahead = (uint64_t{own} + sharers * t) * kBlock;
   if (ahead < p.k)
 #pragma unroll
-    for (int r = 0; r < 2 * R; ++r)
-      if (n0 + 8 * r + g < p.n)
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.b + (n0 + 8 * r + g) * p.b_stride + ahead));
+    for (int h = 0; h < 2; ++h)
+      if (n0 + 8 * h + g < p.n)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.b + (n0 + 8 * h + g) * p.b_stride + ahead));
   aut::dev::pdl_wait();
   aut::dev::pdl_release();
   const uint32_t blocks = static_cast<uint32_t>((p.k + kBlock - 1) / kBlock);
   const uint32_t whole = static_cast<uint32_t>(p.k / kBlock);
   const uint4 zero = make_uint4(0, 0, 0, 0);
-  const uint8_t *b[R][2], *a[T]; // lane (g, t): the codes from 32 t of a block
-  bool has_b[R][2], has_a[T];
+  const uint8_t *b[2], *a[T]; // lane (g, t): the codes from 32 t of a block
+  bool has_b[2], has_a[T];
 #pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint64_t row = n0 + 16 * r + 8 * h + g;
-      has_b[r][h] = row < p.n;
-      b[r][h] = p.b + (has_b[r][h] ? row : 0) * p.b_stride + 32 * t;
-    }
+  for (int h = 0; h < 2; ++h) {
+    const uint64_t row = n0 + 8 * h + g;
+    has_b[h] = row < p.n;
+    b[h] = p.b + (has_b[h] ? row : 0) * p.b_stride + 32 * t;
+  }
 #pragma unroll
   for (int i = 0; i < T; ++i) {
     const uint64_t row = 8 * i + g;
     has_a[i] = row < p.m;
     a[i] = p.a + (has_a[i] ? row : 0) * p.a_stride + 32 * t;
   }
-  float acc[R][T][4] = {};
-  for (uint32_t first = warp; first < blocks; first += 8 * kAhead) {
-    uint4 u[kAhead][R][2][2], w[kAhead][T][2];
+  float acc[T][4] = {};
+  for (uint32_t first = own; first < whole; first += sharers * kAhead) {
+    uint4 u[kAhead][2][2], w[kAhead][T][2];
     float s[kAhead][T][2], column[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const uint32_t block = first + 8 * i;
+      const uint32_t block = first + sharers * i;
       const uint64_t c = uint64_t{block} * kBlock;
       const bool in = block < whole;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+      for (int h = 0; h < 2; ++h) {
+        u[i][h][0] = u[i][h][1] = zero;
+        if (in && has_b[h]) stream_load<Wide>(b[h] + c, u[i][h][0], u[i][h][1]);
+      }
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (half == 0) { // both halves at once
-              u[i][r][h][0] = u[i][r][h][1] = zero;
-              if (in && has_b[r][h]) stream_load<Wide>(b[r][h] + c, u[i][r][h][0], u[i][r][h][1]);
-            }
+      for (int half = 0; half < 2; ++half)
 #pragma unroll
         for (int x = 0; x < T; ++x)
           w[i][x][half] = in && has_a[x]
                               ? __ldg(reinterpret_cast<const uint4 *>(a[x] + c + 16 * half))
                               : zero;
-      }
-      column[i] =
-          block < blocks ? __ldg(p.b_scales + n0 / kBlock + block * p.b_scale_stride) : 0.0f;
+      column[i] = in ? __ldg(p.b_scales + n0 / kBlock + block * p.b_scale_stride) : 0.0f;
 #pragma unroll
       for (int x = 0; x < T; ++x)
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          s[i][x][e] = block < blocks && 8 * x + 2 * t + e < p.m
+          s[i][x][e] = in && 8 * x + 2 * t + e < p.m
                            ? __ldg(p.a_scales + block * p.a_scale_stride + 8 * x + 2 * t + e)
                            : 0.0f;
     }
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const uint32_t block = first + 8 * i;
-      if (block == whole && whole < blocks) { // the last block, cut short by k
+    for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+      for (int x = 0; x < T; ++x) {
+        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const uint64_t c = uint64_t{block} * kBlock + 32 * t + 16 * half;
-#pragma unroll
-          for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-              if (has_b[r][h]) u[i][r][h][half] = load_last(b[r][h] - 32 * t, c, p.k);
-#pragma unroll
-          for (int x = 0; x < T; ++x)
-            if (has_a[x]) w[i][x][half] = load_last(a[x] - 32 * t, c, p.k);
+          const uint4 lo = u[i][0][half], hi = u[i][1][half], v = w[i][x][half];
+          mma<BCode, ACode>(d, lo.x, hi.x, lo.y, hi.y, v.x, v.y);
+          mma<BCode, ACode>(d, lo.z, hi.z, lo.w, hi.w, v.z, v.w);
         }
+        const float s0 = s[i][x][0] * column[i], s1 = s[i][x][1] * column[i];
+        acc[x][0] = fmaf(d[0], s0, acc[x][0]);
+        acc[x][1] = fmaf(d[1], s1, acc[x][1]);
+        acc[x][2] = fmaf(d[2], s0, acc[x][2]);
+        acc[x][3] = fmaf(d[3], s1, acc[x][3]);
       }
+  }
+  // the last block, cut short by k
+  if (whole < blocks && own == whole % sharers) {
+    const float column = p.b_scales[whole * p.b_scale_stride + n0 / kBlock];
 #pragma unroll
-      for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int x = 0; x < T; ++x) {
-          float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint4 lo = u[i][r][0][half], hi = u[i][r][1][half], v = w[i][x][half];
-            mma<BCode, ACode>(d, lo.x, hi.x, lo.y, hi.y, v.x, v.y);
-            mma<BCode, ACode>(d, lo.z, hi.z, lo.w, hi.w, v.z, v.w);
-          }
-          const float s0 = s[i][x][0] * column[i], s1 = s[i][x][1] * column[i];
-          acc[r][x][0] = fmaf(d[0], s0, acc[r][x][0]);
-          acc[r][x][1] = fmaf(d[1], s1, acc[r][x][1]);
-          acc[r][x][2] = fmaf(d[2], s0, acc[r][x][2]);
-          acc[r][x][3] = fmaf(d[3], s1, acc[r][x][3]);
-        }
+    for (int x = 0; x < T; ++x) {
+      float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        const uint64_t c = uint64_t{whole} * kBlock + 32 * t + 16 * half;
+        const uint4 lo = has_b[0] ? load_end(b[0] - 32 * t, c, p.k) : zero;
+        const uint4 hi = has_b[1] ? load_end(b[1] - 32 * t, c, p.k) : zero;
+        const uint4 v = has_a[x] ? load_end(a[x] - 32 * t, c, p.k) : zero;
+        mma<BCode, ACode>(d, lo.x, hi.x, lo.y, hi.y, v.x, v.y);
+        mma<BCode, ACode>(d, lo.z, hi.z, lo.w, hi.w, v.z, v.w);
+      }
+      const float *s = p.a_scales + whole * p.a_scale_stride + 8 * x + 2 * t;
+      const float s0 = 8 * x + 2 * t < p.m ? s[0] * column : 0.0f;
+      const float s1 = 8 * x + 2 * t + 1 < p.m ? s[1] * column : 0.0f;
+      acc[x][0] = fmaf(d[0], s0, acc[x][0]);
+      acc[x][1] = fmaf(d[1], s1, acc[x][1]);
+      acc[x][2] = fmaf(d[2], s0, acc[x][2]);
+      acc[x][3] = fmaf(d[3], s1, acc[x][3]);
     }
   }
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+  for (int x = 0; x < T; ++x)
 #pragma unroll
-    for (int x = 0; x < T; ++x)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        sums[warp][16 * r + 8 * (e / 2) + g][8 * x + 2 * t + e % 2] = acc[r][x][e];
+    for (int e = 0; e < 4; ++e) sums[warp][8 * (e / 2) + g][8 * x + 2 * t + e % 2] = acc[x][e];
   __syncthreads();
-  join_warps<16 * R, 8 * T>(p, sums, 0, n0);
+  if constexpr (Parts == 1) join_warps<16, 8 * T>(p, sums, 0, n0);
+  else join_cluster<16, 8 * T, Parts>(p, sums, n0, rank);
 }
 
 template <class Params>
 aut_status launch(void (*kernel)(Params), uint64_t grid, int max_grid, int threads,
-                  const Params &p, cudaStream_t stream, size_t shared = 0) {
+                  const Params &p, cudaStream_t stream, size_t shared = 0, unsigned cluster = 1) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(grid < static_cast<uint64_t>(max_grid) ? grid : max_grid));
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = shared;
   cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   AUT_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, p));
   return AUT_OK;
 }
 
-template <int ACode, int BCode, bool Wide>
-aut_status gemm_few(aut_workspace *ws, const gemm_params &p, cudaStream_t stream) {
-  if (p.m <= 8)
-    return launch(stream_kernel<ACode, BCode, 1, 1, Wide>, (p.n + 15) / 16, 0x7fffffff, 256, p,
-                  stream);
-  // 32 rows of b to a block where that still gives every SM one
-  if ((p.n + 31) / 32 >= static_cast<uint64_t>(ws->sm_count))
-    return launch(stream_kernel<ACode, BCode, 2, 2, Wide>, (p.n + 31) / 32, 0x7fffffff, 256, p,
-                  stream);
-  return launch(stream_kernel<ACode, BCode, 1, 2, Wide>, (p.n + 15) / 16, 0x7fffffff, 256, p,
-                stream);
+template <int ACode, int BCode, int T, bool Wide>
+aut_status gemm_stream(const gemm_params &p, bool shared, cudaStream_t stream) {
+  const uint64_t groups = (p.n + 15) / 16;
+  return shared ? launch(stream_kernel<ACode, BCode, T, Wide, 4>, 4 * groups, 0x7fffffff, 256, p,
+                         stream, 0, 4)
+                : launch(stream_kernel<ACode, BCode, T, Wide, 1>, groups, 0x7fffffff, 256, p, stream);
 }
 
 template <int ACode, int BCode>
@@ -513,15 +536,24 @@ aut_status gemm_typed(aut_workspace *ws, const gemm_params &p, cudaStream_t stre
   if (!aligned_operands(p, 16) || p.k == 0)
     return launch(rows_kernel<ACode, BCode>, (p.n + 15) / 16 * ((p.m + 7) / 8),
                   64 * ws->max_blocks, 256, p, stream);
-  if (p.m > 16) return gemm_tiles(ws, p, ACode, BCode, stream);
+  const uint64_t groups = (p.n + 15) / 16, at_once = 2 * static_cast<uint64_t>(ws->sm_count);
+  // Few rows of b and a long k: a cluster of four blocks shares k.  Measured: 1 x
+  // 1024 x 16384 4.9 against 7.0 us, 16 x 1024 x 8192 4.9 against 6.5; 8 x 1024 x
+  // 4096 3.4 against 2.8.
+  const bool shared = 4 * groups <= at_once && p.k >= 64 * kBlock;
   // Measured: up to 8 rows streaming is faster than tiles (8 x 8192 x 8192: 15.0
-  // against 16.4 us, 1 x 4096 x 4096: 4.1 against 6.8); up to 16 it is
-  // where b is small (16 x 4096 x 4096: 6.1 against 7.1 us; 8192 x 8192: 19.5
-  // against 16.4).
-  if (p.m > 8 && p.n * p.k >= uint64_t{1} << 25) return gemm_tiles(ws, p, ACode, BCode, stream);
-  return aligned_operands(p, 32) && p.n * p.k < uint64_t{1} << 25
-             ? gemm_few<ACode, BCode, true>(ws, p, stream)
-             : gemm_few<ACode, BCode, false>(ws, p, stream);
+  // against 16.4 us, 1 x 4096 x 4096: 4.1 against 6.8); up to 16 it is where all
+  // of b goes through at once and k is not long (16 x 4096 x 4096: 5.7 against 7.1
+  // us, 10 x 2048 x 8192 6.4 against 8.6; 16 x 16384 x 1024 8.3 against 5.5, 10 x
+  // 2048 x 16000 16.6 against 11.0).
+  if (p.m > 16 || (p.m > 8 && !shared && (groups > at_once || p.k > 64 * kBlock)))
+    return gemm_tiles(ws, p, ACode, BCode, stream);
+  const bool wide = aligned_operands(p, 32) && p.n * p.k < uint64_t{1} << 25;
+  if (p.m <= 8)
+    return wide ? gemm_stream<ACode, BCode, 1, true>(p, shared, stream)
+                : gemm_stream<ACode, BCode, 1, false>(p, shared, stream);
+  return wide ? gemm_stream<ACode, BCode, 2, true>(p, shared, stream)
+              : gemm_stream<ACode, BCode, 2, false>(p, shared, stream);
 }
 
 } // namespace

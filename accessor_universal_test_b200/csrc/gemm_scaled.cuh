@@ -26,6 +26,23 @@ __device__ __forceinline__ void store_out(const gemm_params &p, uint64_t i, uint
   else static_cast<__half *>(p.out)[at] = narrow<__half>(v);
 }
 
+// Of all threads of the cluster's blocks.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\t"
+               "barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// What stands at p in the shared memory of the cluster's block `rank`.
+__device__ __forceinline__ float cluster_load(const float *p, uint32_t rank) {
+  uint32_t a;
+  float v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;"
+      : "=r"(a)
+      : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+
 // Whether every row of both operands starts on a boundary of `bytes`.
 inline bool aligned_operands(const gemm_params &p, uint64_t bytes) {
   return reinterpret_cast<uintptr_t>(p.a) % bytes == 0 && (p.m == 1 || p.a_stride % bytes == 0) &&

@@ -98,7 +98,7 @@ __device__ __forceinline__ uint32_t leader_addr(const void *p) {
 }
 
 // Four floats of shared memory of the cluster's block `rank`.
-__device__ __forceinline__ float4 cluster_load(const float *p, uint32_t rank) {
+__device__ __forceinline__ float4 cluster_load_four(const float *p, uint32_t rank) {
   uint32_t a;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
   float4 v;
@@ -127,12 +127,6 @@ __device__ __forceinline__ bool elected() {
                "selp.u32 %0, 1, 0, p;\n\t}"
                : "=r"(one));
   return one != 0;
-}
-
-// Of all threads of the cluster's blocks.
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\t"
-               "barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // The loads of both blocks of a pair are counted on its first block's barrier.
@@ -750,7 +744,7 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
       float4 u[8];
 #pragma unroll
       for (uint32_t q = 0; q < 8; ++q)
-        if (q < shared_by) u[q] = cluster_load(sums + row * kJoinPitch + column, q);
+        if (q < shared_by) u[q] = cluster_load_four(sums + row * kJoinPitch + column, q);
 #pragma unroll
       for (uint32_t q = 0; q < 8; ++q)
         if (q < shared_by) {

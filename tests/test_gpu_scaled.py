@@ -391,6 +391,18 @@ def test_gemm_keeps_nan_and_infinity_in_their_rows(ws, m):
     np.testing.assert_array_equal(got[np.ix_(rows, columns)], clean[np.ix_(rows, columns)])
 
 
+@pytest.mark.parametrize("m", [1, 8, 9, 16])
+@pytest.mark.parametrize("k", [8191, 8192, 8193, 8207, 8320, 9000, 20011])
+@pytest.mark.parametrize("type", [FP32, FP16])
+def test_gemm_few_rows_share_a_long_k(ws, m, k, type):
+    n = 37 + k % 100
+    a, sa = operand(m, k, ref.E4M3, 1, m)
+    b, sb = operand(n, k, ref.E5M2, 128, k)
+    got = run_gemm(ws, a, sa, b, sb, ref.E4M3, ref.E5M2, type)
+    check_gemm(got, a, sa, b, sb, ref.E4M3, ref.E5M2, type)
+    np.testing.assert_array_equal(run_gemm(ws, a, sa, b, sb, ref.E4M3, ref.E5M2, type), got)
+
+
 @pytest.mark.parametrize("m", [1, 20, 33, 64, 65, 130])
 @pytest.mark.parametrize("k", [1, 2, 3, 5, 126, 127, 129, 131, 255, 383, 640])
 def test_gemm_rows_on_any_boundary(ws, m, k):
