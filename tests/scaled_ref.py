@@ -1,5 +1,5 @@
-"""Plain 64-bit forms of the block-scaled 8-bit operators (numpy), the checker
-of aut_encode_scaled, aut_rms_norm_scaled and aut_gemm_scaled."""
+"""Plain 64-bit forms of the block-scaled 8-bit operators (numpy): what
+aut_encode_scaled, aut_rms_norm_scaled and aut_gemm_scaled are tested against."""
 import numpy as np
 
 BLOCK = 128

@@ -1,4 +1,4 @@
-"""The 64-bit checker of the block-scaled operators against torch's 8-bit
+"""The 64-bit forms of the block-scaled operators against torch's 8-bit
 floats, and the refusals of the C entry points that need no GPU."""
 import numpy as np
 import pytest
