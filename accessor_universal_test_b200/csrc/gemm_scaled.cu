@@ -163,12 +163,12 @@ __global__ void __launch_bounds__(256) rows_kernel(const gemm_params p) {
 // A thread block computes 128 rows of b against 64 rows of a, a warp 32 against
 // 32.  The blocks of k go through shared memory: rows are read as the aligned
 // words that hold them, a line of a row to a warp, moved into place and widened
-// to FP16, which holds every code's value: the matrix instruction for 8-bit
-// operands widens them itself, for every warp that uses them.  The next
-// block's words are under way behind this block's products.  Eight values stand
+// to FP16, which holds every code's value (4096 x 4096 x 1999: 460 us; with the codes
+// as they are, 509, more of whose registers spill).  The next block's words are
+// under way behind this block's products.  Eight values stand
 // at chunk ^ 4 in odd rows, so that eight lanes' reads of two rows meet no bank
-// twice.  Measured at 4096 x 4096 x 1999: 460 us, where the few rows' kernel
-// took 4170 and operands on 16-byte boundaries take about 30.
+// twice.  The few rows' kernel took 4170 us there; operands on 16-byte
+// boundaries take about 30.
 constexpr int kAnyN = 128, kAnyM = 64, kAnyThreads = 256;
 
 struct any_tile {
