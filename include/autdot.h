@@ -386,7 +386,12 @@ aut_status aut_rms_norm_scaled(aut_workspace *ws, int32_t code, int32_t type,
  * a_code with one scale per row (block_rows = 1), b (the weights, one row per
  * output column) codes b_code with block_rows = 128.  The codes' products are
  * summed in FP32 within a block of 128 and then, times both scales, over the
- * blocks.  Codes beyond column k are never read into the product.  Operands
+ * blocks.  The two scales of a block are multiplied with each other first, in
+ * FP32, whatever m: their product should be 0 or a normal number, in magnitude
+ * from 2^-126 to below 2^128.  Below, it has fewer digits or is 0; above, it is
+ * infinite, which a block's sum of 0 turns into NaN.  (Rows of zeros, which
+ * aut_encode_scaled gives the scale 2^-126, are 0 with any scale of b below
+ * 2^128.)  Codes beyond column k are never read into the product.  Operands
  * whose pointers and strides are multiples of 16 bytes take the vectorised
  * paths.  m = 0 or n = 0 does nothing; k = 0 writes zeros. */
 aut_status aut_gemm_scaled(aut_workspace *ws, int32_t a_code, int32_t b_code,
