@@ -13,6 +13,9 @@
 namespace aut {
 // Bound of the bulk-copy kernels' barrier waits: ~2 s of SM clock at 2 GHz.
 constexpr long long kWaitCyclesDefault = 4000000000LL;
+// The shortest bound: copies under way land within a few thousand cycles, so a
+// block whose wait has run out does not leave before its own have.
+constexpr long long kWaitCyclesLeast = 1000000LL;
 } // namespace aut
 
 namespace aut::lib {

@@ -3,6 +3,7 @@
 
 #include "aut/detail/codec_core.hpp"
 
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstdlib>
@@ -634,8 +635,9 @@ aut_status aut_workspace_inject_stall(aut_workspace *ws, uint64_t stall_tile,
   if (wait_cycles > static_cast<uint64_t>(aut::kWaitCyclesDefault))
     return fail(AUT_ERR_INVALID_ARGUMENT, "wait_cycles above the default bound");
   ws->stall_tile = stall_tile;
-  ws->wait_cycles = wait_cycles == 0 ? aut::kWaitCyclesDefault
-                                     : static_cast<long long>(wait_cycles);
+  ws->wait_cycles =
+      wait_cycles == 0 ? aut::kWaitCyclesDefault
+                       : std::max(aut::kWaitCyclesLeast, static_cast<long long>(wait_cycles));
   return AUT_OK;
 }
 

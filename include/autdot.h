@@ -188,7 +188,8 @@ aut_status aut_workspace_status(aut_workspace *ws, uint32_t *status,
  * bounded waits).  Until called again, the bulk-copy (TMA) DOT kernels
  * launched through `ws` arm the ring stage of tile `stall_tile` of every
  * pair without issuing its copies, and bound every barrier wait by
- * `wait_cycles` SM clock cycles (0: the default, ~2 s).  The wait for that
+ * `wait_cycles` SM clock cycles (0: the default, ~2 s; at least 1000000, so
+ * that a block's own copies land within it).  The wait for that
  * stage therefore runs out: the block lets its other copies land, sets
  * AUT_STATUS_WAIT_TIMEOUT and the DOT's result is NaN.  No copy is left in
  * flight, nothing waits without a bound, and the context stays usable.
