@@ -669,7 +669,8 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
           acc[c] = make_float2(__int_as_float(0x7fffffff), __int_as_float(0x7fffffff));
       }
       if constexpr (Split) {
-        // all of this block's products are done: the ring is free for its sums
+        // all of this block's products are done: the ring is free for its sums (if
+        // a wait has run out, they are written again once its loads have landed)
         float *sums = reinterpret_cast<float *>(ring) + row * kJoinPitch + stripe * kColumns;
 #pragma unroll
         for (int c = 0; c < kColumns / 2; c += 2)
@@ -733,6 +734,11 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
       bar_wait(&drained, 0, p.wait_cycles, &none);
     }
     __syncthreads();
+    if constexpr (Split) {
+      float *sums = reinterpret_cast<float *>(ring);
+      for (int at = threadIdx.x; at < kTileM * kJoinPitch; at += shape::kThreads)
+        sums[at] = __int_as_float(0x7fffffff);
+    }
   }
   if constexpr (Split) {
     __syncwarp();

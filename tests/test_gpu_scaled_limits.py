@@ -14,7 +14,7 @@ INFINITY = 0x7C  # E5M2
 # uncut tiles of 32, 64, 128 and 256 columns, rows on any boundary (stride 1)
 INFINITE = [(1, 300, 5120, 0), (12, 300, 5120, 0), (64, 1024, 5120, 0), (32, 1024, 5120, 0),
             (87, 256, 2333, 0), (100, 1000, 3000, 0), (150, 300, 2304, 0), (33, 520, 640, 0),
-            (300, 10300, 2000, 0), (129, 9000, 1500, 0), (20, 300, 2000, 1), (70, 300, 2000, 1)]
+            (300, 10300, 2000, 0), (300, 6500, 1999, 0), (20, 300, 2000, 1), (70, 300, 2000, 1)]
 
 
 @pytest.mark.parametrize("size", INFINITE)
@@ -51,7 +51,7 @@ def test_an_infinite_code_gives_an_infinite_result(ws, size, side):
 # cluster, tiles of 32 (cut and uncut), 64, 128 and 256 columns, any boundary
 RANGES = [(1, 300, 700, 0), (8, 40, 9000, 0), (12, 300, 700, 0), (64, 1024, 5120, 0),
           (33, 520, 640, 0), (129, 700, 3000, 0), (150, 3000, 700, 0), (300, 10300, 700, 0),
-          (9, 300, 700, 1), (70, 300, 700, 1)]
+          (300, 6500, 700, 0), (9, 300, 700, 1), (70, 300, 700, 1)]
 
 
 def large_codes(rows, columns, seed):

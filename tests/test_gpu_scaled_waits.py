@@ -12,8 +12,10 @@ from test_gpu_scaled import FP32, check_gemm, operand
 pytestmark = pytest.mark.gpu
 
 OFF = 2 ** 64 - 1
-# tiles of 32 columns (cut and uncut), 64 (cut), 128 and 256
-SIZES = [(64, 1024, 5120), (33, 520, 640), (129, 700, 3000), (150, 3000, 2000), (300, 10300, 2000)]
+# tiles of 32 columns (cut and uncut), 64 (cut and uncut), 128, and 256 (rows of the
+# result on 16 bytes, and not)
+SIZES = [(64, 1024, 5120), (33, 520, 640), (129, 700, 3000), (150, 3000, 2000), (300, 10300, 2000),
+         (300, 6500, 1999), (300, 6501, 1999)]
 
 
 class Product:
@@ -64,3 +66,21 @@ def test_a_bound_of_one_cycle_is_no_fault_of_a_dot(ws, orc):
         ws.inject_stall()
     dot, size = oracle_dot(orc, "e8m0", 1 << 20)
     assert normalized_error(got, dot, size) <= TOL[0]
+
+
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("block", [0, 3])
+def test_what_a_block_had_to_write_is_nan(size, block):
+    """Every thread block misses one load of its first tile, so nothing that it or
+    the blocks it joins with write is a number.  (Of more tiles to a block, the
+    later ones too.)"""
+    w = _lib.Workspace(0)
+    product = Product(w, *size)
+    w.inject_stall(block, 1)
+    got = product()
+    assert w.status() == _lib.STATUS_WAIT_TIMEOUT
+    assert np.isnan(got).all()
+    w.inject_stall()
+    product.check(product())
+    assert w.status() == 0
+    w.close()
