@@ -729,7 +729,8 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
                      &none);
       }
     }
-    if (warp >= shape::kProductWarp && lane == 0 && rank == 0) {
+    // by the lane that issued them: a commit counts its own thread's products
+    if (warp >= shape::kProductWarp && rank == 0 && elected()) {
       mma_commit<Pair>(&drained);
       bar_wait(&drained, 0, p.wait_cycles, &none);
     }
