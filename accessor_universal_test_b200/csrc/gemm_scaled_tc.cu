@@ -633,6 +633,7 @@ __global__ void __launch_bounds__(tile_shape<BN, Pair>::kThreads, 1)
           break;
         }
         if (at + shape::kBatch == kScaleBatch || block + shape::kBatch >= blocks) {
+          __syncwarp(); // of all lanes' reads: a vote orders no memory
           if (lane == 0) bar_arrive(&scales_used[slot]);
           ++batch;
         }
