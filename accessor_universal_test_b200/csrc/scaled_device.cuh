@@ -85,9 +85,10 @@ struct block_scale {
 // needs no case of its own.  The division by the constant F is a product with
 // 1 / F and Markstein's correction (the residual is exact in one FMA).  The
 // reciprocal starts from the hardware's approximation r, within an ulp; with
-// e = 1 - scale r, exact in one FMA, 1 / scale = r + r (e + e^2) up to r e^3.  So
-// rounded, inverse is 1 / scale rounded down (checked with all 2^23 fractions of a
-// scale and every r within an ulp), and what is left of it is made the same way.
+// e = 1 - scale r, one FMA, 1 / scale = r + r (e + e^2) up to r e^3.  So rounded,
+// inverse is 1 / scale rounded down (checked with all 2^23 fractions of a scale
+// and every r within an ulp of the nearest value), and what is left of it is made
+// the same way, now with an exact e.
 template <int Code> __device__ __forceinline__ block_scale scale_of(float largest) {
   constexpr float f = largest_code<Code>(), reciprocal = 1.0f / f;
   block_scale s;
