@@ -152,32 +152,23 @@ __device__ __forceinline__ float without_infinity(float v) {
   return fabsf(v) <= 3.40282347e38f ? v : __int_as_float(0x7fffffff);
 }
 
-// Encodes the chunk: codes into the row, scales into scales[block * stride].
-// All lanes of the warp take part.
+// Encodes a chunk of numbers with the largest magnitudes m of the lane's values
+// (of either half of them, or of all in both): codes into the row, scales into
+// scales[block * stride], times back.  All lanes of the warp take part.
 template <int Code, bool Vec>
-__device__ __forceinline__ void encode_chunk(float2 (&v)[4], uint32_t chunk, int lane,
-                                             uint32_t columns, uint8_t *row, float *scales,
-                                             uint64_t scale_stride) {
-  constexpr int kHalves = Vec ? 1 : 2;
-  float m[2] = {largest_of(v[0], v[1]), largest_of(v[2], v[3])};
-  if (Vec) m[0] = m[1] = fmaxf(m[0], m[1]);
-  // Rare, and not worth a test for every value: an infinity.
-  if (__any_sync(0xffffffffu, fmaxf(m[0], m[1]) > 3.40282347e38f)) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      v[j] = make_float2(without_infinity(v[j].x), without_infinity(v[j].y));
-    m[0] = largest_of(v[0], v[1]), m[1] = largest_of(v[2], v[3]);
-    if (Vec) m[0] = fmaxf(m[0], m[1]);
-  }
+__device__ __forceinline__ void encode_numbers(const float2 (&v)[4], const float (&m)[2],
+                                               uint32_t chunk, int lane, uint32_t columns,
+                                               uint8_t *row, float *scales,
+                                               uint64_t scale_stride, const float (&back)[2]) {
   uint32_t codes[4]; // two each
   block_scale s;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    if (h < kHalves) {
+    if (h < (Vec ? 1 : 2)) {
       s = scale_of<Code>(Vec ? half_warp_max(m[h], lane) : warp_max(m[h]));
       const uint32_t block = chunk * 2 + (Vec ? lane / 16 : h);
       if ((Vec ? lane % 16 : lane) == 0 && block * kBlock < columns)
-        scales[block * scale_stride] = s.scale;
+        scales[block * scale_stride] = s.scale * back[h];
     }
 #pragma unroll
     for (int j = 2 * h; j < 2 * h + 2; ++j) {
@@ -204,6 +195,39 @@ __device__ __forceinline__ void encode_chunk(float2 (&v)[4], uint32_t chunk, int
   }
 }
 
+// The same of any values.  Exact: with scales above kLargeScale too (of a norm's
+// values, which are within some ulp of theirs, no quotient's rounding is that exact).
+template <int Code, bool Vec, bool Exact>
+__device__ __forceinline__ void encode_chunk(float2 (&v)[4], uint32_t chunk, int lane,
+                                             uint32_t columns, uint8_t *row, float *scales,
+                                             uint64_t scale_stride) {
+  float m[2] = {largest_of(v[0], v[1]), largest_of(v[2], v[3])}, back[2] = {1.0f, 1.0f};
+  if (Vec) m[0] = m[1] = fmaxf(m[0], m[1]);
+  // Rare, and not worth a test for every value: an infinity or a large scale.
+  if (__any_sync(0xffffffffu, fmaxf(m[0], m[1]) > (Exact ? kLargeScale : 3.40282347e38f))) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      v[j] = make_float2(without_infinity(v[j].x), without_infinity(v[j].y));
+    m[0] = largest_of(v[0], v[1]), m[1] = largest_of(v[2], v[3]);
+    if (Vec) m[0] = m[1] = fmaxf(m[0], m[1]);
+    if constexpr (Exact) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const bool large = (Vec ? half_warp_max(m[h], lane) : warp_max(m[h])) > kLargeScale;
+        const float down = large ? kDown : 1.0f;
+        back[h] = large ? kUp : 1.0f;
+        m[h] *= down;
+#pragma unroll
+        for (int j = 2 * h; j < 2 * h + 2; ++j) v[j] = mul2(v[j], make_float2(down, down));
+      }
+      // code of its own: a factor of every scale made all others 6 % slower
+      encode_numbers<Code, Vec>(v, m, chunk, lane, columns, row, scales, scale_stride, back);
+      return;
+    }
+  }
+  encode_numbers<Code, Vec>(v, m, chunk, lane, columns, row, scales, scale_stride, back);
+}
+
 // ---- encode by rows ---------------------------------------------------------------
 // Block (c, y) takes chunk c of the row groups y, y + gridDim.y, ... of 16
 // rows, a warp two rows of a group; the next group's values are loaded before
@@ -219,6 +243,7 @@ constexpr int kEncodeRows = 16;
 template <int Type, int Code, bool Vec>
 __global__ void __launch_bounds__(256) encode_rows_kernel(const encode_params p) {
   using T = element_t<Type>;
+  constexpr bool kExact = Type != AUT_TYPE_FP16; // FP16 has no values that large
   aut::dev::pdl_wait();
   aut::dev::pdl_release();
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
@@ -240,9 +265,9 @@ __global__ void __launch_bounds__(256) encode_rows_kernel(const encode_params p)
     x += x_step;
     if (row + step < p.rows) next[0] = load_raw<Vec>(x, chunk, lane, columns);
     if (row + step + 8 < p.rows) next[1] = load_raw<Vec>(x + 8 * p.x_stride, chunk, lane, columns);
-    encode_chunk<Code, Vec>(v[0], chunk, lane, columns, codes, p.scales + row, p.scale_stride);
+    encode_chunk<Code, Vec, kExact>(v[0], chunk, lane, columns, codes, p.scales + row, p.scale_stride);
     if (two)
-      encode_chunk<Code, Vec>(v[1], chunk, lane, columns, codes + 8 * p.code_stride,
+      encode_chunk<Code, Vec, kExact>(v[1], chunk, lane, columns, codes + 8 * p.code_stride,
                               p.scales + row + 8, p.scale_stride);
   }
 }
@@ -362,8 +387,10 @@ __global__ void __launch_bounds__(tile_of<element_t<Type>>::kThreads,
     if (lane == 0) part[turn][warp] = largest;
     __syncthreads();
     largest = warp_max(part[turn][lane % tile::kWarps]);
-    const bool infinite = largest > 3.40282347e38f; // rare; the same for all
-    if (infinite) {
+    // rare, and the same for all: an infinity or a large scale
+    const bool large = largest > kLargeScale;
+    float down = 1.0f, back = 1.0f;
+    if (large) {
       __syncthreads();
       largest = 0.0f;
 #pragma unroll
@@ -378,9 +405,10 @@ __global__ void __launch_bounds__(tile_of<element_t<Type>>::kThreads,
       if (lane == 0) part[turn][warp] = largest;
       __syncthreads();
       largest = warp_max(part[turn][lane % tile::kWarps]);
+      if (largest > kLargeScale) largest *= kDown, down = kDown, back = kUp;
     }
     const block_scale s = scale_of<Code>(largest);
-    if (threadIdx.x == 0) p.scales[block_now * p.scale_stride + group_now] = s.scale;
+    if (threadIdx.x == 0) p.scales[block_now * p.scale_stride + group_now] = s.scale * back;
     const uint64_t first = group_now * kBlock + warp;
     const uint32_t column = block_now * kBlock + lane_column;
     uint8_t *to = p.codes + first * p.code_stride + column;
@@ -389,10 +417,11 @@ __global__ void __launch_bounds__(tile_of<element_t<Type>>::kThreads,
     for (int r = 0; r < tile::kRows; ++r, to += tile::kWarps * p.code_stride) {
       float2 v[2];
       widen_four(now[r], v);
-      if (infinite) {
+      if (large) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
-          v[j] = make_float2(without_infinity(v[j].x), without_infinity(v[j].y));
+          v[j] = mul2(make_float2(without_infinity(v[j].x), without_infinity(v[j].y)),
+                      make_float2(down, down));
       }
       const uint32_t codes = four_codes<Code>(quotient(v[0], s), quotient(v[1], s));
       const bool has_row = first + r * tile::kWarps < p.rows;
@@ -507,7 +536,7 @@ __global__ void __launch_bounds__(Threads < 128 ? 128 : Threads,
 #pragma unroll
         for (int j = 0; j < 4; ++j) h[i][j] = mul2(h[i][j], w[j]);
       }
-      encode_chunk<Code, Vec>(h[i], chunk, lane, columns, p.e.codes + row * p.e.code_stride,
+      encode_chunk<Code, Vec, false>(h[i], chunk, lane, columns, p.e.codes + row * p.e.code_stride,
                               p.e.scales + row, p.e.scale_stride);
     }
   }
@@ -566,7 +595,7 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const norm_params p) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) h[j] = mul2(h[j], s[j]);
     }
-    encode_chunk<Code, false>(h, chunk, lane, columns, p.e.codes + row * p.e.code_stride,
+    encode_chunk<Code, false, false>(h, chunk, lane, columns, p.e.codes + row * p.e.code_stride,
                               p.e.scales + row, p.e.scale_stride);
   }
 }

@@ -110,12 +110,16 @@ template <int Code> __device__ __forceinline__ block_scale scale_of(float larges
 // that decides; all 712 pairs of fractions of scale and value that lie within 2^-43 of
 // one were checked and come out right (with the roundings of scale_of, not with
 // others).  The rest is not negative, so a zero keeps its sign.  Two operations for
-// two values, where a division takes about ten for each.
-// (For scales above 2^100 the rest loses digits: the quotient is then within
-// 2 ulp.)
+// two values, where a division takes about ten for each.  Scales are at most
+// kLargeScale here: the rest of a larger one's inverse would lose digits below the
+// normal range.
 __device__ __forceinline__ float2 quotient(float2 x, const block_scale &s) {
   return fma2(x, make_float2(s.inverse, s.inverse), mul2(x, make_float2(s.rest, s.rest)));
 }
+
+// Blocks with larger values are encoded times kDown, their scale times kUp.  What that
+// takes below the normal range has a quotient that rounds to zero.
+constexpr float kLargeScale = 0x1p100f, kDown = 0x1p-64f, kUp = 0x1p64f;
 
 // |v| for a block's largest magnitude: infinities and NaN do not count.
 __device__ __forceinline__ float finite_magnitude(float v) {

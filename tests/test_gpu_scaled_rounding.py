@@ -70,7 +70,7 @@ def check_bits(got, x, code, block_rows):
 
 
 @pytest.mark.parametrize("code", [ref.E4M3, ref.E5M2])
-@pytest.mark.parametrize("exponent", [-126, -110, -60, 0, 60, 90, 99])
+@pytest.mark.parametrize("exponent", [-126, -110, -60, 0, 60, 90, 99, 100, 101, 105, 110])
 def test_quotients_beside_a_tie(ws, code, exponent):
     x = blocks_of(code, exponent)
     assert x.shape[0] > 20
@@ -82,6 +82,20 @@ def test_quotients_beside_a_tie(ws, code, exponent):
     x = np.concatenate([x[::128], x[::128]], 1)
     check_bits(run_encode(ws, x, FP32, code, 1, x_stride=257, stride=259, offset=1),
                x.astype(np.float32), code, 1)
+
+
+@pytest.mark.parametrize("code", [ref.E4M3, ref.E5M2])
+@pytest.mark.parametrize("type", [FP32, BF16])
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_large_scales(ws, code, type, block_rows):
+    """Blocks of values up to 2^128 beside blocks of small ones, and both in one."""
+    x = values(384, 700, 3)
+    x[:, 128:256] *= 2.0 ** 120
+    x[130:, 300:500] *= 2.0 ** 104
+    x[:, 600:] *= np.exp2(np.random.default_rng(4).integers(-120, 110, (384, 100)))
+    x[3, 140], x[200, 140] = np.inf, -np.inf
+    x = rounded(np.clip(x, -3e38, 3e38, where=np.isfinite(x), out=x), type)
+    check_bits(run_encode(ws, x, type, code, block_rows), x, code, block_rows)
 
 
 @pytest.mark.parametrize("type", [FP32, BF16, FP16])
