@@ -9,7 +9,10 @@ the norm that makes them or by ``encode``::
     a, stream = scaled.rms_norm(ws, x, gain, residual=stream)
     y = scaled.matmul(ws, a, w)                              # x.dtype out
 
-Every call runs on torch's current stream of the tensors' device.
+Every call runs on torch's current stream of the tensors' device.  None of them
+is differentiated: where gradients are recorded, tensors that require one are
+refused.  What a call writes in place counts as changed for torch, so a backward
+pass that needs the old values says so.
 """
 from __future__ import annotations
 
@@ -50,7 +53,15 @@ def _stream(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+def _written(*tensors: torch.Tensor) -> None:
+    """Tells torch of tensors that a call has written through their pointers."""
+    torch.autograd.graph.increment_version(tensors)
+
+
 def _check(name: str, t: torch.Tensor, ws: _lib.Workspace, shape=None, dtype=None) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, which these calls do not make "
+                         "(detach it, or call under torch.no_grad())")
     if t.device != torch.device("cuda", ws.device):
         raise ValueError(f"{name} is on {t.device}, the workspace on cuda:{ws.device}")
     if t.dtype not in TYPES or (dtype is not None and t.dtype != dtype):
@@ -83,6 +94,7 @@ def encode(ws: _lib.Workspace, values: torch.Tensor, code: int = _lib.FP8_E4M3,
     ws.encode_scaled(code, TYPES[values.dtype], block_rows, values.data_ptr(), values.stride(0),
                      rows, columns, out.storage.data_ptr(), out.storage.stride(0),
                      out.scales.data_ptr(), out.scales.stride(0), _stream(values))
+    _written(out.storage, out.scales)
     return out
 
 
@@ -106,7 +118,11 @@ def rms_norm(ws: _lib.Workspace, x: torch.Tensor, weight: torch.Tensor | None = 
                        0 if weight is None else weight.data_ptr(), eps, rows, columns,
                        out.storage.data_ptr(), out.storage.stride(0), out.scales.data_ptr(),
                        out.scales.stride(0), _stream(x))
-    return out, x if residual is None else residual
+    _written(out.storage, out.scales)
+    if residual is None:
+        return out, x
+    _written(residual)
+    return out, residual
 
 
 def matmul(ws: _lib.Workspace, a: Scaled, b: Scaled, dtype: torch.dtype = torch.bfloat16,
@@ -128,4 +144,5 @@ def matmul(ws: _lib.Workspace, a: Scaled, b: Scaled, dtype: torch.dtype = torch.
                    a.scales.data_ptr(), a.scales.stride(0), b.storage.data_ptr(),
                    b.storage.stride(0), b.scales.data_ptr(), b.scales.stride(0), a.rows, b.rows,
                    a.columns, out.data_ptr(), out.stride(0), _stream(out))
+    _written(out)
     return out

@@ -74,3 +74,22 @@ def test_tensor_calls_refuse_what_does_not_fit():
         scaled.matmul(ws, a, scaled.Scaled(300, 128, block_rows=128))
     with pytest.raises(ValueError, match="workspace on cuda:0"):
         scaled.matmul(ws, a, b)
+
+
+def test_tensor_calls_refuse_to_drop_a_gradient():
+    """Refused before anything else where gradients are recorded, and only there."""
+    from accessor_universal_test_b200 import scaled
+
+    class Handle:
+        device = 0
+
+    ws = Handle()
+    grad = torch.zeros(4, 256, requires_grad=True)
+    for call in (lambda: scaled.encode(ws, grad), lambda: scaled.rms_norm(ws, grad),
+                 lambda: scaled.encode(ws, grad * 2)):
+        with pytest.raises(ValueError, match="requires a gradient"):
+            call()
+    with torch.no_grad(), pytest.raises(ValueError, match="workspace on cuda:0"):
+        scaled.encode(ws, grad)
+    with pytest.raises(ValueError, match="workspace on cuda:0"):
+        scaled.encode(ws, grad.detach())
