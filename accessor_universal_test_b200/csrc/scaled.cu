@@ -695,11 +695,14 @@ aut_status norm_rows(aut_workspace *ws, const norm_params &p, cudaStream_t strea
   const uint64_t columns = p.e.columns;
   if (columns <= 256) return norm_launch<Type, Code, Vec, 32, 1>(ws, p, stream);
   if (columns <= 1024) return norm_launch<Type, Code, Vec, 128, 1>(ws, p, stream);
-  if (columns <= 8192 &&
-      (Type == AUT_TYPE_FP32 || p.e.rows <= static_cast<uint64_t>(ws->sm_count)))
+  if (columns <= 8192) {
+    if constexpr (Type != AUT_TYPE_FP32) {
+      if (p.e.rows > static_cast<uint64_t>(ws->sm_count))
+        return columns <= 4096 ? norm_launch<Type, Code, Vec, 256, 2>(ws, p, stream)
+                               : norm_launch<Type, Code, Vec, 512, 2>(ws, p, stream);
+    }
     return norm_launch<Type, Code, Vec, 1024, 1>(ws, p, stream);
-  if (columns <= 4096) return norm_launch<Type, Code, Vec, 256, 2>(ws, p, stream);
-  if (columns <= 8192) return norm_launch<Type, Code, Vec, 512, 2>(ws, p, stream);
+  }
   return norm_launch<Type, Code, Vec, 1024, 2>(ws, p, stream);
 }
 
