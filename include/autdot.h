@@ -372,7 +372,9 @@ aut_status aut_encode_scaled(aut_workspace *ws, int32_t code, int32_t type,
  * x, residual, residual_out and weight[columns] have the type `type`;
  * residual and residual_out share residual_stride.  residual_out may be
  * residual itself, or x where both strides are equal; it may not overlap
- * them otherwise.  The mean is summed in FP32. */
+ * them otherwise.  The mean is summed in FP32: a row whose sum of squares
+ * passes FP32's largest value (values of about 2^64 on) is encoded as zeros,
+ * and one of zeros with eps = 0 as NaN. */
 aut_status aut_rms_norm_scaled(aut_workspace *ws, int32_t code, int32_t type,
                                const void *x, uint64_t x_stride,
                                const void *residual, void *residual_out,

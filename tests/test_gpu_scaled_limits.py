@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import scaled_ref as ref
-from test_gpu_scaled import FP32, check_gemm, operand, run_gemm
+from test_gpu_scaled import FP32, check_gemm, check_norm, operand, run_gemm, run_norm, values
 
 pytestmark = pytest.mark.gpu
 
@@ -160,3 +160,17 @@ def test_scales_that_are_zero_or_not_finite(ws, size):
         got = run_gemm(ws, a, sa, b, sb, ref.E4M3, ref.E4M3, FP32, **layout_of(k, off))
         inside = np.arange(n) // 128 == 1
         assert np.isnan(got[:, inside]).all() and np.isfinite(got[:, ~inside]).all()
+
+
+@pytest.mark.parametrize("columns", [200, 512, 5001, 16392])
+def test_norm_of_rows_beyond_the_range_of_their_squares(ws, columns):
+    """Zeros where the sum of squares overflows; just below, values as any other."""
+    x = values(4, columns, 3, spread=0.1)
+    x[1] *= 2.0 ** 70
+    x[2] = 2.0 ** 54
+    got, after = run_norm(ws, x, None, None, 1e-5, FP32, ref.E4M3, into="new")
+    assert (got[0][1] == 0).all() and (got[1][:, 1] == np.float32(2.0 ** -126)).all()
+    np.testing.assert_array_equal(after, x.astype(np.float32))
+    rest = [0, 2, 3]
+    check_norm((got[0][rest], got[1][:, rest]), after[rest], x[rest], None, None, 1e-5, FP32,
+               ref.E4M3)
