@@ -163,8 +163,8 @@ __global__ void __launch_bounds__(256) rows_kernel(const gemm_params p) {
 // A thread block computes 128 rows of b against 64 rows of a, a warp 32 against
 // 32.  The blocks of k go through shared memory: rows are read as the aligned
 // words that hold them, a line of a row to a warp, moved into place and widened
-// to FP16, which holds every code's value (4096 x 4096 x 1999: 460 us; with the codes
-// as they are, 509, more of whose registers spill).  The next block's words are
+// to FP16, which holds every code's value (4096 x 4096 x 1999: 462 us; with the codes
+// as they are, 509, more of whose registers spill: here 92 bytes a thread).  The next block's words are
 // under way behind this block's products.  Eight values stand
 // at chunk ^ 4 in odd rows, so that eight lanes' reads of two rows meet no bank
 // twice.  The few rows' kernel took 4170 us there; operands on 16-byte
@@ -350,11 +350,18 @@ __global__ void __launch_bounds__(kAnyThreads, 2) any_tiles_kernel(const gemm_pa
 // of k, kAhead at a time, all of whose loads are issued before the first product.  Measured (m x n x k, GB/s of
 // codes): 1 x 4096 x 4096 with kAhead 1, 2, 3, 4: 3387, 3640, 2963, 2729;
 // 8 x 8192 x 8192: 3763, 4364, 4063, 4004 (registers: fewer blocks to an SM);
-// keeping the next kAhead blocks' loads under way behind each product: 4181.
+// keeping the next kAhead blocks' loads under way behind each product: 4181.  (b
+// partly in the second-level cache; from memory 1 x 4096 x 4096 takes 4.6 us, 3.7
+// TB/s, and 8 x 8192 x 8192 15.9.)  For 9 to 16 rows 12 to 40 bytes a thread spill.
 
-// 32 codes of a row, in one load or two.  Measured: one load is faster where b is
-// small (1 x 4096 x 4096: 4.1 against 4.7 us), two where it is large (8 x 8192 x
-// 8192: 15.0 against 16.1 us).
+// 32 codes of a row, in one load or two.  Measured with three b in turn, one load
+// against two: faster for b below 2^25 codes, which stays in the second-level cache
+// (8 x 2048 x 2048 1.96 and 2.14 us, 8 x 4096 x 4096 4.02 and 4.60, 8 x 1024 x 16384
+// 5.03 and 5.60), slower where part of a larger one does (8 x 8192 x 8192 15.7 and
+// 14.9, 1 x 16384 x 8192 26.8 and 25.9).  With b read from memory every time, one
+// load is as fast or faster at all sizes up to 8 rows (1 x 4096 x 4096 4.56 and 4.72,
+// 8 x 8192 x 8192 15.4 and 15.9, 1 x 28672 x 4096 22.5 and 25.1; 16 x 4096 x 8192
+// 12.4 and 12.1).
 template <bool Wide>
 __device__ __forceinline__ void stream_load(const uint8_t *p, uint4 &v, uint4 &w) {
   if constexpr (Wide) {

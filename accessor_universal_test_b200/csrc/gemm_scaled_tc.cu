@@ -348,7 +348,9 @@ template <int BN, bool Pair> struct tile_shape {
   static constexpr int kRingBytes = (BN == 256 ? 192 : BN == 128 ? 200 : 204) * 1024;
   // Epilogue warps: four to a scheduler for the wide tiles, so that some read
   // tensor memory while others add (4096 x 8192 x 8192: 865 cycles a block of
-  // k and tile where two to a scheduler took 962; the products alone, 513).
+  // k and tile where two to a scheduler took 962; the products alone, 513).  The
+  // pair's 96 registers a thread leave 16 bytes to local memory, 52 where results
+  // are turned.
   static constexpr int kEpilogueWarps = BN >= 128 ? 16 : 8;
   static constexpr int kParts = kEpilogueWarps / 4; // of the columns
   static constexpr int kLoadWarp = kEpilogueWarps, kScaleWarp = kEpilogueWarps + 1,
@@ -912,7 +914,7 @@ aut_status gemm_tiles(aut_workspace *ws, const gemm_params &g, int a_code, int b
   // a start of about 3 us, for every block of k that an SM goes through 0.14 to
   // 0.18 us with 32 columns (32 and 128 x 4096 x 4096: 7.1 and 8.9 us), 0.2 with
   // 64 (16 x 8192 x 8192: 16.4), 0.3 with 128 (256 x 8192 x 8192: 24.6), 0.54
-  // for a pair on 256 x 256 (4096 x 8192 x 8192: 258), and to join S parts of k
+  // for a pair on 256 x 256 (4096 x 8192 x 8192: 256, at 1.6 GHz), and to join S parts of k
   // 0.5 + 0.4 S us (64 x 1024 x 8192 with 64 columns, S = 1, 2, 4: 14.9, 10.3,
   // 7.5 us).  What a last step goes through beyond its blocks is not counted: it
   // loads nothing where k has ended, and with whole steps in the price 40 sizes of

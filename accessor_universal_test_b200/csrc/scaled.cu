@@ -235,8 +235,8 @@ __device__ __forceinline__ void encode_chunk(float2 (&v)[4], uint32_t chunk, int
 // group are neighbours: the scales of one column block fill whole lines.
 // Bound by memory, with the schedulers busy two thirds of the time (the search
 // for the maximum, the scale and the conversions).  Measured, copy bandwidth
-// 6.55 TB/s: 4096 x 8192 BF16 18.1 us (5.6 TB/s), FP32 26.4 (6.4); 4096 x 5001 FP32
-// 18.6 (5.6), FP16 19.9 (3.1: eight loads and eight stores of a lane for
+// 6.55 TB/s: 4096 x 8192 BF16 17.9 us (5.6 TB/s), FP32 26.2 (6.4); 4096 x 5001 FP32
+// 18.3 (5.6), FP16 20.1 (3.1: eight loads and eight stores of a lane for
 // one of each where rows start on 16 bytes).
 constexpr int kEncodeRows = 16;
 
@@ -276,9 +276,9 @@ __global__ void __launch_bounds__(256) encode_rows_kernel(const encode_params p)
 // A block holds a tile in registers (16 a thread: 32 values of 16 bits, 16 of
 // 32), so the tile is read once, and loads its next one before it encodes this
 // one.  Vec: lane l holds the columns 4 l .., a multiple of 4 in all; else
-// l + 32 j (see above).  Measured: 8192 x 8192 FP32 51.3 us (6.5 TB/s), 8192 x 5120
-// BF16 24.6 (5.1), 8191 x 5001 FP32 35.4 (5.8), FP16 40.4 (3.0; with a test of row
-// and column at each value of every tile 51.7).
+// l + 32 j (see above).  Measured: 8192 x 8192 FP32 51.1 us (6.6 TB/s), BF16 36.7
+// (5.5), 8192 x 5120 BF16 24.3 (5.2), 8191 x 5001 FP32 35.1 (5.8), FP16 40.1 (3.1;
+// with a test of row and column at each value of every tile 51.7).
 template <class T> struct tile_of {
   static constexpr int kThreads = sizeof(T) == 4 ? 1024 : 512;
   static constexpr int kWarps = kThreads / 32;
@@ -452,10 +452,12 @@ __device__ __forceinline__ float warp_sum(float v) {
 // weight stays in registers over the rows of a block.  The next row's values
 // are loaded before this one's are summed and encoded.  Threads = 32: four
 // rows to a block of 128.  Bound by memory; one barrier a row, which the other
-// blocks of the SM fill.  Measured with a residual in place: 4096 x 8192 BF16 39.9 us
-// (5.9 TB/s), 4096 x 4096 FP32 35.6 (6.1), 4096 x 5001 FP32 47.3 (5.6), BF16 55.2 (2.6:
+// blocks of the SM fill.  Measured with a residual in place: 4096 x 8192 BF16 40.0 us
+// (5.9 TB/s), 4096 x 4096 FP32 35.9 (6.1), 4096 x 5001 FP32 48.2 (5.5), BF16 55.5 (2.6:
 // the same count of instructions as FP32 for half the bytes, and stores of 64
-// bytes that begin and end within a sector), 1 x 4096 BF16 1.7.
+// bytes that begin and end within a sector), 1 x 4096 BF16 1.6.  FP32 rows of 8193 to
+// 16384 columns do not fit: 120 bytes a thread go to local memory (240 off 16-byte
+// boundaries) and 4096 x 12288 takes 132 us (5.0 TB/s); 16-bit rows there, 24 to 32.
 template <int Type, int Code, bool Vec, int Threads, int Chunks>
 __global__ void __launch_bounds__(Threads < 128 ? 128 : Threads,
                                   65536 / (Threads < 256 ? 48 : Threads < 512 ? 80 : 64) /
@@ -544,7 +546,8 @@ __global__ void __launch_bounds__(Threads < 128 ? 128 : Threads,
 
 // Rows too long for the registers: read twice, the second time mostly from
 // the second-level cache.  A value is read and, in place, written by one and
-// the same thread.
+// the same thread.  Element by element on any boundary: 4096 x 18432 BF16 155 us
+// (3.4 TB/s of what has to move).
 template <int Type, int Code>
 __global__ void __launch_bounds__(1024) norm_long_kernel(const norm_params p) {
   using T = element_t<Type>;
