@@ -177,7 +177,8 @@ class Workspace:
 
     def inject_stall(self, stall_tile: int = 2**64 - 1, wait_cycles: int = 0) -> None:
         """Failure-detection test hook: the bulk-copy kernels withhold the
-        copies of tile `stall_tile`, so their bounded wait runs out."""
+        copies of tile `stall_tile`, so their bounded wait runs out (after
+        wait_cycles, at least a million)."""
         check(load().aut_workspace_inject_stall(self.handle, stall_tile, wait_cycles))
 
     def dot_batched(self, fmt, layout, accum, x_ptr, y_ptr, n, batch, stride_bytes,

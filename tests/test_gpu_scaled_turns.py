@@ -77,7 +77,7 @@ def test_norm_leaves_its_boundaries_one_at_a_time(ws, type, columns, layout):
 @pytest.mark.parametrize("which", ["weight", "residual", "residual_out"])
 def test_norm_with_one_pointer_off_its_boundary(ws, type, which):
     import torch
-    from test_gpu_scaled import TORCH, Encoded, device_matrix, rounded
+    from test_gpu_scaled import TORCH, Encoded, device_matrix
     rows, columns = 11, 304
     x, residual = values(rows, columns, 5), values(rows, columns, 6)
     weight = 1 + 0.1 * np.random.default_rng(4).standard_normal(columns)
